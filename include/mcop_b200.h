@@ -55,6 +55,7 @@ enum {
   MCOP_DEVERR_POSITION = 16, /* RoPE position outside [0, max_position) */
   MCOP_DEVERR_SLOT = 17,     /* paged-cache slot >= num_blocks * block_size */
   MCOP_DEVERR_KV_INDEX = 18, /* store_kv: slot id outside [0, num_slots) or cache position outside [0, max_len) */
+  MCOP_DEVERR_SEQUENCE = 19, /* sequence bounds that descend or leave the buffer */
   MCOP_DEVERR_SELFTEST = 99  /* recorded by mcop_selftest_wait_timeout */
 };
 
@@ -222,6 +223,74 @@ int mcop_rope_kv_store_i8_paged(const int64_t* positions, void* query, void* key
                                 int head_size, int rot_dim, int64_t query_stride, int64_t key_stride,
                                 int64_t value_stride, int block_size, int64_t num_blocks, int is_neox,
                                 int dtype, mcop_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Part 2, the paged cache after it is written: dynamic int8 store, read-back, attention.  No counterpart in the reference
+ * (mcoplib leaves the cache's readers to other libraries).
+ *
+ * The caches are [num_blocks, block_size, kv_heads, head_size] with strides in elements for block, in-block position and
+ * head, shared by the K and the V cache; head_size a multiple of 16 of at most 256, every row 16-byte aligned, at most
+ * 2^31 - 1 slots.  scale_mode 0: the cache holds the element type (bf16 or f16); 1: int8 with k_scale, v_scale fp32
+ * [kv_heads] (what mcop_rope_kv_store_i8_paged writes); 2: int8 with k_scale, v_scale fp32 [num_blocks, block_size, kv_heads]
+ * (what mcop_reshape_and_cache_dynamic_i8 writes).  value = code * scale.
+ * block_tables int32 [batch, table_stride], of whose rows the first max_blocks entries count: position p of sequence b is
+ * at offset p % block_size of block block_tables[b, p / block_size].  Entries behind a sequence's last page are not read.
+ * A page outside [0, num_blocks) hides its tokens (MCOP_DEVERR_SLOT), a length beyond the table is cut (MCOP_DEVERR_KV_INDEX),
+ * a sequence whose bounds descend or leave the buffer is skipped (MCOP_DEVERR_SEQUENCE).
+ * ---------------------------------------------------------------------------------------------- */
+
+/* Quantise as the cache is written.  No counterpart in the reference.  For every (token, head) row of key and value
+ * [tokens, kv_heads, head_size] (contiguous heads, token strides given; dtype f32, bf16 or f16):
+ *   scale = max|x| / 127 (fp32 division),  code = the integer nearest to x / scale (the real quotient, ties to even),
+ * codes to the int8 caches and scale to k_scale / v_scale [num_blocks, block_size, kv_heads] at slot_mapping[t] (negative =
+ * skip; a slot >= num_blocks * block_size is skipped and reported, MCOP_DEVERR_SLOT).  A row of zeros gets scale 0 and codes 0, a row
+ * with a NaN or an infinity scale NaN and codes 0.  Slots should be distinct: two tokens with one slot leave a mixture. */
+int mcop_reshape_and_cache_dynamic_i8(const void* key, const void* value, int64_t key_stride, int64_t value_stride,
+                                      int8_t* key_cache, int8_t* value_cache, int64_t block_stride, int64_t page_stride,
+                                      int64_t head_stride, float* k_scale, float* v_scale, const int64_t* slot_mapping,
+                                      int64_t tokens, int kv_heads, int head_size, int block_size, int64_t num_blocks,
+                                      int dtype, mcop_stream_t stream);
+
+/* Read a batch of sequences back out of the cache.  No counterpart in the reference.
+ * key_out, value_out [tokens, kv_heads, head_size] contiguous: row cu_seq_lens[b] + p = position p of sequence b, times its
+ * scale, rounded once to dtype (bf16, f16; f32 with an int8 cache; dtype is the cache's own type with scale_mode 0).
+ * cu_seq_lens int32 [batch + 1].  Rows before cu_seq_lens[0], behind cu_seq_lens[batch] and of bad pages keep what they held. */
+int mcop_gather_and_dequant_cache(void* key_out, void* value_out, const void* key_cache, const void* value_cache,
+                                  int64_t block_stride, int64_t page_stride, int64_t head_stride, const float* k_scale,
+                                  const float* v_scale, int scale_mode, const int32_t* block_tables, int64_t table_stride,
+                                  int max_blocks, const int32_t* cu_seq_lens, int batch, int64_t tokens, int kv_heads,
+                                  int head_size, int block_size, int64_t num_blocks, int dtype, mcop_stream_t stream);
+
+/* Attention of one new token per sequence over its cached tokens.  No counterpart in the reference.
+ * query, out [batch, q_heads, head_size] (token and head strides in elements, rows 16-byte aligned, dtype bf16 or f16);
+ * query head h reads KV head h / (q_heads / kv_heads).  The token of sequence b is its last cached one: it sees the last
+ * `window` positions (0: all) of [0, seq_lens[b]).  out = softmax(scale * q . k) v; lse (fp32 [batch, q_heads], may be NULL)
+ * = ln sum exp(scale * q . k).  A sequence of length 0 gets out = 0 and lse = -inf.  scale must be positive.
+ * The lengths stay on the device, so one captured graph serves any lengths.  workspace: 16-byte aligned, at least
+ * mcop_paged_attention_decode_workspace_bytes(); needs no initialisation, must not be shared by calls that overlap. */
+size_t mcop_paged_attention_decode_workspace_bytes(int batch, int q_heads, int kv_heads, int head_size);
+int mcop_paged_attention_decode(void* out, int64_t out_token_stride, int64_t out_head_stride, float* lse, const void* query,
+                                int64_t query_token_stride, int64_t query_head_stride, const void* key_cache,
+                                const void* value_cache, int64_t block_stride, int64_t page_stride, int64_t head_stride,
+                                const float* k_scale, const float* v_scale, int scale_mode, const int32_t* block_tables,
+                                int64_t table_stride, int max_blocks, const int32_t* seq_lens, int batch, int q_heads,
+                                int kv_heads, int head_size, int block_size, int64_t num_blocks, float scale, int window,
+                                int dtype, void* workspace, size_t workspace_bytes, mcop_stream_t stream);
+
+/* Attention of a chunk of new tokens per sequence over its cached tokens, the new ones among them.
+ * No counterpart in the reference.  query, out [tokens, q_heads, head_size]: rows cu_seqlens_q[b] .. cu_seqlens_q[b + 1] (int32 [batch + 1]) are
+ * sequence b's last q_len tokens, so new token i stands at position pos = seq_lens[b] - q_len + i.  It sees the positions
+ * j <= pos (causal != 0; otherwise all) with j > pos - window (window 0: no lower bound).  A token that sees nothing gets
+ * out = 0 and lse = -inf.  Rows of out and lse outside the sequences keep what they held.  The rest as for decode. */
+size_t mcop_paged_attention_chunk_workspace_bytes(int64_t tokens, int batch, int q_heads, int kv_heads, int head_size);
+int mcop_paged_attention_chunk(void* out, int64_t out_token_stride, int64_t out_head_stride, float* lse, const void* query,
+                               int64_t query_token_stride, int64_t query_head_stride, const void* key_cache,
+                               const void* value_cache, int64_t block_stride, int64_t page_stride, int64_t head_stride,
+                               const float* k_scale, const float* v_scale, int scale_mode, const int32_t* block_tables,
+                               int64_t table_stride, int max_blocks, const int32_t* seq_lens, const int32_t* cu_seqlens_q,
+                               int batch, int64_t tokens, int q_heads, int kv_heads, int head_size, int block_size,
+                               int64_t num_blocks, float scale, int causal, int window, int dtype, void* workspace,
+                               size_t workspace_bytes, mcop_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------------
  * Part 3 - MoE routing, dispatch (scatter + quant) and combine (gather)

@@ -35,6 +35,12 @@ SIGNATURES = {
     "mcop_reshape_and_cache_flash": (I32, [P, P, I64, I64, P, P, I64, I64, I64, P, I64, I32, I32, I32, I64, I32, P]),
     "mcop_reshape_and_cache": (I32, [P, P, I64, I64, P, P, P, I64, I32, I32, I32, I32, I64, I32, P]),
     "mcop_rope_kv_store_i8_paged": (I32, [P, P, P, P, P, I32, I64, P, P, P, P, P, I64, I32, I32, I32, I32, I64, I64, I64, I32, I64, I32, I32, P]),
+    "mcop_reshape_and_cache_dynamic_i8": (I32, [P, P, I64, I64, P, P, I64, I64, I64, P, P, P, I64, I32, I32, I32, I64, I32, P]),
+    "mcop_gather_and_dequant_cache": (I32, [P, P, P, P, I64, I64, I64, P, P, I32, P, I64, I32, P, I32, I64, I32, I32, I32, I64, I32, P]),
+    "mcop_paged_attention_decode_workspace_bytes": (SZ, [I32, I32, I32, I32]),
+    "mcop_paged_attention_decode": (I32, [P, I64, I64, P, P, I64, I64, P, P, I64, I64, I64, P, P, I32, P, I64, I32, P, I32, I32, I32, I32, I32, I64, F32, I32, I32, P, SZ, P]),
+    "mcop_paged_attention_chunk_workspace_bytes": (SZ, [I64, I32, I32, I32, I32]),
+    "mcop_paged_attention_chunk": (I32, [P, I64, I64, P, P, I64, I64, P, P, I64, I64, I64, P, P, I32, P, I64, I32, P, P, I32, I64, I32, I32, I32, I32, I64, F32, I32, I32, I32, P, SZ, P]),
     "mcop_moe_softmax_topk": (I32, [P, P, P, I64, I32, I32, P]),
     "mcop_grouped_topk": (I32, [P, P, P, P, I64, I32, I32, I32, I32, I32, C.c_double, I32, I32, I32, P]),
     "mcop_topk_softmax": (I32, [P, P, P, P, I64, I32, I32, I32, I32, P]),
@@ -61,7 +67,7 @@ GATHER_NOALLOC_SCRATCH_BYTES = 4 << 20
 
 F32_CODE, BF16_CODE, F16_CODE = 0, 1, 2
 # codes of mcop_device_error()
-DEVERR_POSITION, DEVERR_SLOT, DEVERR_KV_INDEX, DEVERR_SELFTEST = 16, 17, 18, 99
+DEVERR_POSITION, DEVERR_SLOT, DEVERR_KV_INDEX, DEVERR_SEQUENCE, DEVERR_SELFTEST = 16, 17, 18, 19, 99
 
 _lib = None
 

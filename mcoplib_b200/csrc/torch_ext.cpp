@@ -450,6 +450,158 @@ void rope_kv_store_int8(Tensor& positions, Tensor& query, Tensor& key, Tensor& v
                                        is_neox ? 1 : 0, dtype_code(query, "rope_kv_store_int8"), cur_stream()));
 }
 
+// ---------------------------------------------------------------- part 2, the readers of the paged cache (additions of this build)
+
+// A dimension of one entry has no stride of its own: whatever the tensor says there is never multiplied by anything but 0.
+int64_t stride_of(const Tensor& t, int64_t dim) { return t.size(dim) > 1 ? t.stride(dim) : 0; }
+
+// What the paged-cache operators ask of a cache pair; returns the scale mode of the C ABI.
+int check_paged_cache(const Tensor& key_cache, const Tensor& value_cache, const std::optional<Tensor>& k_scale, const std::optional<Tensor>& v_scale,
+                      at::ScalarType type) {
+  check_cuda(key_cache, "key_cache");
+  TORCH_CHECK(key_cache.dim() == 4 && key_cache.sizes() == value_cache.sizes() && stride_of(key_cache, 0) == stride_of(value_cache, 0) &&
+                  stride_of(key_cache, 1) == stride_of(value_cache, 1) && stride_of(key_cache, 2) == stride_of(value_cache, 2) &&
+                  key_cache.scalar_type() == value_cache.scalar_type(),
+              "key_cache and value_cache must be [num_blocks, block_size, kv_heads, head_size] and share type and layout");
+  TORCH_CHECK(key_cache.stride(3) == 1, "the heads of the caches must be contiguous");
+  TORCH_CHECK(key_cache.device() == value_cache.device(), "the caches must be on one device");
+  if (key_cache.scalar_type() != at::kChar) {
+    TORCH_CHECK(key_cache.scalar_type() == type, "the cache must be int8 or of the type of the other tensors");
+    TORCH_CHECK(!k_scale.has_value() && !v_scale.has_value(), "scales go with an int8 cache only");
+    return 0;
+  }
+  TORCH_CHECK(k_scale.has_value() && v_scale.has_value(), "an int8 cache needs k_scale and v_scale");
+  TORCH_CHECK(k_scale->scalar_type() == at::kFloat && v_scale->scalar_type() == at::kFloat && k_scale->is_contiguous() && v_scale->is_contiguous() &&
+                  k_scale->sizes() == v_scale->sizes() && k_scale->device() == key_cache.device() && v_scale->device() == key_cache.device(),
+              "k_scale and v_scale must be contiguous fp32 tensors of one shape on the caches' device");
+  if (k_scale->dim() == 1) {
+    TORCH_CHECK(k_scale->size(0) == key_cache.size(2), "scales per head must be [kv_heads]");
+    return 1;
+  }
+  TORCH_CHECK(k_scale->dim() == 3 && k_scale->size(0) == key_cache.size(0) && k_scale->size(1) == key_cache.size(1) &&
+                  k_scale->size(2) == key_cache.size(2),
+              "scales must be [kv_heads] or [num_blocks, block_size, kv_heads]");
+  return 2;
+}
+
+void check_index(const Tensor& t, const char* name, const Tensor& like, int64_t dim) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, " must be on the caches' device");
+  TORCH_CHECK(t.scalar_type() == at::kInt && t.dim() == dim && (t.size(dim - 1) <= 1 || t.stride(dim - 1) == 1), name,
+              " must be int32 with ", dim, " dimension(s), the last one contiguous");
+}
+
+const float* opt_float(const std::optional<Tensor>& t) { return t.has_value() ? t->data_ptr<float>() : nullptr; }
+
+// K and V rows to int8 codes with one scale per (token, head), made as they are written
+void reshape_and_cache_dynamic_int8(const Tensor& key, const Tensor& value, Tensor& key_cache, Tensor& value_cache, Tensor& k_scale, Tensor& v_scale,
+                                    const Tensor& slot_mapping) {
+  MCOP_DEBUG_CALL("reshape_and_cache_dynamic_int8", key, value, key_cache, value_cache, k_scale, v_scale, slot_mapping);
+  check_cuda(key, "key");
+  TORCH_CHECK(key_cache.scalar_type() == at::kChar, "the caches must be int8");
+  TORCH_CHECK(check_paged_cache(key_cache, value_cache, k_scale, v_scale, at::kChar) == 2, "scales must be [num_blocks, block_size, kv_heads]");
+  TORCH_CHECK(key.dim() == 3 && value.sizes() == key.sizes() && value.scalar_type() == key.scalar_type() && key.size(1) == key_cache.size(2) &&
+                  key.size(2) == key_cache.size(3),
+              "key and value must be [tokens, kv_heads, head_size] of one type");
+  TORCH_CHECK(key.stride(2) == 1 && value.stride(2) == 1 && (key.size(1) == 1 || (key.stride(1) == key.size(2) && value.stride(1) == value.size(2))),
+              "heads of key/value must be contiguous");
+  TORCH_CHECK(slot_mapping.scalar_type() == at::kLong && slot_mapping.dim() == 1 && slot_mapping.is_contiguous(), "slot_mapping must be int64 [tokens]");
+  TORCH_CHECK(key.device() == key_cache.device() && value.device() == key_cache.device() && slot_mapping.device() == key_cache.device(),
+              "all tensors must be on the caches' device");
+  const int64_t tokens = slot_mapping.size(0);
+  TORCH_CHECK(key.size(0) >= tokens, "key and value must hold a row for every slot");
+  const c10::cuda::OptionalCUDAGuard guard(device_of(key_cache));
+  check_rc(mcop_reshape_and_cache_dynamic_i8(key.data_ptr(), value.data_ptr(), stride_of(key, 0), stride_of(value, 0), key_cache.data_ptr<int8_t>(),
+                                             value_cache.data_ptr<int8_t>(), stride_of(key_cache, 0), stride_of(key_cache, 1), stride_of(key_cache, 2),
+                                             k_scale.data_ptr<float>(), v_scale.data_ptr<float>(), slot_mapping.data_ptr<int64_t>(), tokens,
+                                             (int)key.size(1), (int)key.size(2), (int)key_cache.size(1), key_cache.size(0),
+                                             dtype_code(key, "reshape_and_cache_dynamic_int8"), cur_stream()));
+}
+
+// The rows of a batch of sequences out of the cache, packed
+void gather_and_dequant_cache(Tensor& key_out, Tensor& value_out, const Tensor& key_cache, const Tensor& value_cache, const Tensor& block_tables,
+                              const Tensor& cu_seq_lens, std::optional<Tensor> k_scale, std::optional<Tensor> v_scale) {
+  MCOP_DEBUG_CALL("gather_and_dequant_cache", key_out, value_out, key_cache, value_cache, block_tables, cu_seq_lens, k_scale, v_scale);
+  const int mode = check_paged_cache(key_cache, value_cache, k_scale, v_scale, key_out.scalar_type());
+  TORCH_CHECK(key_out.dim() == 3 && value_out.sizes() == key_out.sizes() && value_out.scalar_type() == key_out.scalar_type() &&
+                  key_out.is_contiguous() && value_out.is_contiguous() && key_out.size(1) == key_cache.size(2) && key_out.size(2) == key_cache.size(3),
+              "key_out and value_out must be contiguous [tokens, kv_heads, head_size] of one type");
+  TORCH_CHECK(key_out.device() == key_cache.device() && value_out.device() == key_cache.device(), "all tensors must be on the caches' device");
+  check_index(block_tables, "block_tables", key_cache, 2);
+  check_index(cu_seq_lens, "cu_seq_lens", key_cache, 1);
+  const int64_t batch = block_tables.size(0);
+  TORCH_CHECK(cu_seq_lens.size(0) == batch + 1, "cu_seq_lens must hold batch + 1 entries");
+  const c10::cuda::OptionalCUDAGuard guard(device_of(key_cache));
+  check_rc(mcop_gather_and_dequant_cache(key_out.data_ptr(), value_out.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), stride_of(key_cache, 0),
+                                         stride_of(key_cache, 1), stride_of(key_cache, 2), opt_float(k_scale), opt_float(v_scale), mode,
+                                         block_tables.data_ptr<int32_t>(), stride_of(block_tables, 0),
+                                         (int)block_tables.size(1), cu_seq_lens.data_ptr<int32_t>(), (int)batch, key_out.size(0),
+                                         (int)key_cache.size(2), (int)key_cache.size(3), (int)key_cache.size(1), key_cache.size(0),
+                                         dtype_code(key_out, "gather_and_dequant_cache"), cur_stream()));
+}
+
+// Checks shared by the two attention operators; returns the scale mode.
+int check_attention(const Tensor& out, const Tensor& query, const Tensor& key_cache, const Tensor& value_cache, const Tensor& block_tables,
+                    const Tensor& seq_lens, const std::optional<Tensor>& k_scale, const std::optional<Tensor>& v_scale, int64_t window,
+                    const std::optional<Tensor>& lse) {
+  check_cuda(query, "query");
+  TORCH_CHECK(query.scalar_type() == at::kBFloat16 || query.scalar_type() == at::kHalf, "query must be bf16 or f16");
+  const int mode = check_paged_cache(key_cache, value_cache, k_scale, v_scale, query.scalar_type());
+  TORCH_CHECK(query.dim() == 3 && out.sizes() == query.sizes() && out.scalar_type() == query.scalar_type() && query.stride(2) == 1 && out.stride(2) == 1,
+              "query and out must be [tokens, q_heads, head_size] of one type with contiguous heads");
+  TORCH_CHECK(query.device() == key_cache.device() && out.device() == key_cache.device(), "all tensors must be on the caches' device");
+  TORCH_CHECK(query.size(2) == key_cache.size(3) && key_cache.size(2) > 0 && query.size(1) % key_cache.size(2) == 0,
+              "query heads must be a multiple of the caches' heads, of their size");
+  check_index(block_tables, "block_tables", key_cache, 2);
+  check_index(seq_lens, "seq_lens", key_cache, 1);
+  TORCH_CHECK(seq_lens.size(0) == block_tables.size(0), "seq_lens and block_tables must hold one entry per sequence");
+  TORCH_CHECK(window >= 0 && window <= INT32_MAX, "window must be >= 0 (0: none)");
+  if (lse.has_value())
+    TORCH_CHECK(lse->scalar_type() == at::kFloat && lse->is_contiguous() && lse->dim() == 2 && lse->size(0) == query.size(0) &&
+                    lse->size(1) == query.size(1) && lse->device() == key_cache.device(),
+                "lse must be contiguous fp32 [tokens, q_heads]");
+  return mode;
+}
+
+// One new token per sequence over its cached tokens
+void paged_attention_decode(Tensor& out, const Tensor& query, const Tensor& key_cache, const Tensor& value_cache, const Tensor& block_tables,
+                            const Tensor& seq_lens, double scale, std::optional<Tensor> k_scale, std::optional<Tensor> v_scale, int64_t window,
+                            std::optional<Tensor> lse) {
+  MCOP_DEBUG_CALL("paged_attention_decode", out, query, key_cache, value_cache, block_tables, seq_lens, scale, k_scale, v_scale, window, lse);
+  const int mode = check_attention(out, query, key_cache, value_cache, block_tables, seq_lens, k_scale, v_scale, window, lse);
+  TORCH_CHECK(query.size(0) == seq_lens.size(0), "query must hold one token per sequence");
+  const c10::cuda::OptionalCUDAGuard guard(device_of(query));
+  const int batch = (int)query.size(0), q_heads = (int)query.size(1), kv_heads = (int)key_cache.size(2), head_size = (int)query.size(2);
+  Tensor ws = scratch_bytes(mcop_paged_attention_decode_workspace_bytes(batch, q_heads, kv_heads, head_size), query);
+  check_rc(mcop_paged_attention_decode(out.data_ptr(), stride_of(out, 0), stride_of(out, 1), lse.has_value() ? lse->data_ptr<float>() : nullptr,
+                                       query.data_ptr(), stride_of(query, 0), stride_of(query, 1), key_cache.data_ptr(), value_cache.data_ptr(),
+                                       stride_of(key_cache, 0), stride_of(key_cache, 1), stride_of(key_cache, 2), opt_float(k_scale), opt_float(v_scale), mode,
+                                       block_tables.data_ptr<int32_t>(), stride_of(block_tables, 0),
+                                       (int)block_tables.size(1), seq_lens.data_ptr<int32_t>(), batch, q_heads, kv_heads, head_size,
+                                       (int)key_cache.size(1), key_cache.size(0), (float)scale, (int)window,
+                                       dtype_code(query, "paged_attention_decode"), ws.data_ptr(), (size_t)ws.numel(), cur_stream()));
+}
+
+// A chunk of new tokens per sequence over its cached tokens
+void paged_attention_chunk(Tensor& out, const Tensor& query, const Tensor& key_cache, const Tensor& value_cache, const Tensor& block_tables,
+                           const Tensor& seq_lens, const Tensor& cu_seqlens_q, double scale, std::optional<Tensor> k_scale,
+                           std::optional<Tensor> v_scale, bool causal, int64_t window, std::optional<Tensor> lse) {
+  MCOP_DEBUG_CALL("paged_attention_chunk", out, query, key_cache, value_cache, block_tables, seq_lens, cu_seqlens_q, scale, k_scale, v_scale, causal, window, lse);
+  const int mode = check_attention(out, query, key_cache, value_cache, block_tables, seq_lens, k_scale, v_scale, window, lse);
+  check_index(cu_seqlens_q, "cu_seqlens_q", key_cache, 1);
+  TORCH_CHECK(cu_seqlens_q.size(0) == seq_lens.size(0) + 1, "cu_seqlens_q must hold batch + 1 entries");
+  const c10::cuda::OptionalCUDAGuard guard(device_of(query));
+  const int batch = (int)seq_lens.size(0), q_heads = (int)query.size(1), kv_heads = (int)key_cache.size(2), head_size = (int)query.size(2);
+  Tensor ws = scratch_bytes(mcop_paged_attention_chunk_workspace_bytes(query.size(0), batch, q_heads, kv_heads, head_size), query);
+  check_rc(mcop_paged_attention_chunk(out.data_ptr(), stride_of(out, 0), stride_of(out, 1), lse.has_value() ? lse->data_ptr<float>() : nullptr,
+                                      query.data_ptr(), stride_of(query, 0), stride_of(query, 1), key_cache.data_ptr(), value_cache.data_ptr(),
+                                      stride_of(key_cache, 0), stride_of(key_cache, 1), stride_of(key_cache, 2), opt_float(k_scale), opt_float(v_scale), mode,
+                                      block_tables.data_ptr<int32_t>(), stride_of(block_tables, 0),
+                                      (int)block_tables.size(1), seq_lens.data_ptr<int32_t>(), cu_seqlens_q.data_ptr<int32_t>(), batch,
+                                      query.size(0), q_heads, kv_heads, head_size, (int)key_cache.size(1), key_cache.size(0), (float)scale,
+                                      causal ? 1 : 0, (int)window, dtype_code(query, "paged_attention_chunk"), ws.data_ptr(), (size_t)ws.numel(),
+                                      cur_stream()));
+}
+
 // ---------------------------------------------------------------- part 3
 
 // mcoplib.op.moe_softmax_topk (op/moe_softmax_topk.cu:216-235)
@@ -1016,6 +1168,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("fused_silu_mul_dq_quant", &fused_silu_mul_dq_quant);
   // additions of this build (no reference counterpart)
   m.def("rope_kv_store_int8", &rope_kv_store_int8);
+  m.def("reshape_and_cache_dynamic_int8", &reshape_and_cache_dynamic_int8, py::arg("key"), py::arg("value"), py::arg("key_cache"),
+        py::arg("value_cache"), py::arg("k_scale"), py::arg("v_scale"), py::arg("slot_mapping"));
+  m.def("gather_and_dequant_cache", &gather_and_dequant_cache, py::arg("key_out"), py::arg("value_out"), py::arg("key_cache"),
+        py::arg("value_cache"), py::arg("block_tables"), py::arg("cu_seq_lens"), py::arg("k_scale") = py::none(), py::arg("v_scale") = py::none());
+  m.def("paged_attention_decode", &paged_attention_decode, py::arg("out"), py::arg("query"), py::arg("key_cache"), py::arg("value_cache"),
+        py::arg("block_tables"), py::arg("seq_lens"), py::arg("scale"), py::arg("k_scale") = py::none(), py::arg("v_scale") = py::none(),
+        py::arg("window") = 0, py::arg("lse") = py::none());
+  m.def("paged_attention_chunk", &paged_attention_chunk, py::arg("out"), py::arg("query"), py::arg("key_cache"), py::arg("value_cache"),
+        py::arg("block_tables"), py::arg("seq_lens"), py::arg("cu_seqlens_q"), py::arg("scale"), py::arg("k_scale") = py::none(),
+        py::arg("v_scale") = py::none(), py::arg("causal") = true, py::arg("window") = 0, py::arg("lse") = py::none());
   m.def("moe_gather_weighted", &moe_gather_weighted, py::arg("y"), py::arg("row2tok"), py::arg("topk_ids"), py::arg("topk_weights"),
         py::arg("experts_token_start"), py::arg("out"), py::arg("accumulate"), py::arg("tok2row") = py::none());
   // torch-library functions also reachable directly (same objects the dispatcher calls)
@@ -1081,4 +1243,20 @@ TORCH_LIBRARY(MCOP_TORCH_NS_CACHE, cache_ops) {
       "reshape_and_cache_flash(Tensor key, Tensor value, Tensor! key_cache, Tensor! value_cache, Tensor slot_mapping, "
       "str kv_cache_dtype, Tensor k_scale, Tensor v_scale) -> ()");
   cache_ops.impl("reshape_and_cache_flash", torch::kCUDA, &reshape_and_cache_flash);
+  cache_ops.def(
+      "reshape_and_cache_dynamic_int8(Tensor key, Tensor value, Tensor! key_cache, Tensor! value_cache, Tensor! k_scale, "
+      "Tensor! v_scale, Tensor slot_mapping) -> ()");
+  cache_ops.impl("reshape_and_cache_dynamic_int8", torch::kCUDA, &reshape_and_cache_dynamic_int8);
+  cache_ops.def(
+      "gather_and_dequant_cache(Tensor! key_out, Tensor! value_out, Tensor key_cache, Tensor value_cache, Tensor block_tables, "
+      "Tensor cu_seq_lens, Tensor? k_scale=None, Tensor? v_scale=None) -> ()");
+  cache_ops.impl("gather_and_dequant_cache", torch::kCUDA, &gather_and_dequant_cache);
+  cache_ops.def(
+      "paged_attention_decode(Tensor! out, Tensor query, Tensor key_cache, Tensor value_cache, Tensor block_tables, Tensor seq_lens, "
+      "float scale, Tensor? k_scale=None, Tensor? v_scale=None, int window=0, Tensor!? lse=None) -> ()");
+  cache_ops.impl("paged_attention_decode", torch::kCUDA, &paged_attention_decode);
+  cache_ops.def(
+      "paged_attention_chunk(Tensor! out, Tensor query, Tensor key_cache, Tensor value_cache, Tensor block_tables, Tensor seq_lens, "
+      "Tensor cu_seqlens_q, float scale, Tensor? k_scale=None, Tensor? v_scale=None, bool causal=True, int window=0, Tensor!? lse=None) -> ()");
+  cache_ops.impl("paged_attention_chunk", torch::kCUDA, &paged_attention_chunk);
 }
