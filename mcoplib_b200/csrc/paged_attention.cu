@@ -1,75 +1,8 @@
-// Attention of new tokens over the paged KV cache.
-//
-// New token i of a sequence with q_len new tokens and len cached ones (the new ones are cached already) stands at
-// position  pos = len - q_len + i  and sees the positions
-//     [max(0, window ? pos - window + 1 : 0), causal ? pos + 1 : len)  clipped to [0, len).
-// Over those, with s_j = scale * (q . k_j):   out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),   lse = m + ln sum_j exp(s_j - m).
-// A token that sees nothing gets out = 0 and lse = -inf.  The scales of an int8 cache never touch the codes: the K scale multiplies
-// the logit, the V scale the weight, both in fp32.
-#include "paged_cache.cuh"
-#include "tma_pipe.cuh"
+// Attention over the paged cache: the entry points, and the kernel for any head size.
+#include "paged_attention.cuh"
 
 namespace mcop {
 namespace {
-
-struct AttnArgs {
-  PagedCache c;
-  const void* q;
-  void* out;
-  float* lse;  // [tokens, q_heads] or null
-  int64_t q_token, q_head, o_token, o_head;
-  const int32_t* seq_lens;
-  const int32_t* cu;  // null: one new token per sequence
-  int batch, tokens, q_heads, head_size, scale_mode;
-  float scale;
-  int causal, window;
-  int* err;
-};
-
-struct Seq {
-  int q0, qn, len;  // first new token, number of new tokens, cached tokens
-};
-
-// Bounds of sequence b, checked: what the caller's tensors say is never turned into an address beyond the buffers.
-__device__ __forceinline__ Seq sequence(const AttnArgs& a, int b) {
-  Seq s;
-  s.q0 = a.cu ? a.cu[b] : b;
-  const int q1 = a.cu ? a.cu[b + 1] : b + 1;
-  s.qn = q1 - s.q0;
-  if (s.q0 < 0 || q1 < s.q0 || q1 > a.tokens) {
-    report(a.err, MCOP_DEVERR_SEQUENCE);
-    s.q0 = s.qn = 0;
-  }
-  s.len = a.seq_lens[b];
-  const int64_t room = (int64_t)a.c.max_blocks * a.c.block_size;
-  if (s.len < 0 || s.len > room) {
-    report(a.err, MCOP_DEVERR_KV_INDEX);
-    s.len = s.len < 0 ? 0 : (int)room;
-  }
-  return s;
-}
-
-// Positions [lo, hi) that new token i of a sequence sees.
-__device__ __forceinline__ void span(const AttnArgs& a, const Seq& s, int i, int& lo, int& hi) {
-  const int pos = s.len - s.qn + i;
-  hi = a.causal ? min(s.len, max(0, pos + 1)) : s.len;
-  lo = a.window > 0 && pos >= a.window ? pos - a.window + 1 : 0;
-}
-
-// Slot of position `pos` of sequence b, or -1 (reported) where the table names a page that the cache does not have.
-__device__ __forceinline__ int slot_of(const AttnArgs& a, int b, int pos) {
-  const int page = pos / a.c.block_size;
-  const int block = a.c.tables[b * a.c.table_stride + page];
-  if (block < 0 || block >= a.c.num_blocks) {
-    report(a.err, MCOP_DEVERR_SLOT);
-    return -1;
-  }
-  return block * a.c.block_size + (pos - page * a.c.block_size);
-}
-__device__ __forceinline__ int64_t row_of(const PagedCache& c, int slot, int head) {
-  const int block = slot / c.block_size;
-  return block * c.block_stride + (slot - block * c.block_size) * c.page_stride + head * c.head_stride;
-}
 
 // ---------------------------------------------------------------------------------------------
 // Any head size up to 256: one warp per (new token, query head), 32 positions at a time.  A lane forms the whole logit of one
@@ -170,6 +103,10 @@ int check_args(const char* what, const AttnArgs& a, int64_t tokens, int dtype) {
                MCOP_ERR_ARGUMENT, "%s: query and output rows must be 16-byte aligned", what);
   MCOP_REQUIRE(a.c.max_blocks >= 0 && a.c.table_stride >= 0 && (int64_t)a.c.max_blocks * a.c.block_size <= INT32_MAX,
                MCOP_ERR_ARGUMENT, "%s: block table too wide", what);
+  // rows are addressed in units of 16 bytes with 32 bits
+  const double span = (double)a.c.num_blocks * a.c.block_stride + (double)a.c.block_size * a.c.page_stride + (double)a.c.kv_heads * a.c.head_stride;
+  MCOP_REQUIRE(a.c.block_stride >= 0 && a.c.page_stride >= 0 && a.c.head_stride >= 0 && span * (a.scale_mode ? 1 : 2) < 0x1p36, MCOP_ERR_UNSUPPORTED,
+               "%s: a cache may span at most 64 GB, with strides >= 0", what);
   MCOP_REQUIRE(a.window >= 0, MCOP_ERR_ARGUMENT, "%s: negative window", what);
   MCOP_REQUIRE(a.scale > 0.f && a.scale <= FLT_MAX, MCOP_ERR_ARGUMENT, "%s: the scale must be positive", what);
   return MCOP_OK;
@@ -192,7 +129,9 @@ int launch_rows(const char* what, const AttnArgs& a, int dtype, cudaStream_t st)
 
 using namespace mcop;
 
-extern "C" size_t mcop_paged_attention_decode_workspace_bytes(int batch, int q_heads, int kv_heads, int head_size) { return 0; }
+extern "C" size_t mcop_paged_attention_decode_workspace_bytes(int batch, int q_heads, int kv_heads, int head_size) {
+  return batch > 0 && kv_heads > 0 && q_heads > 0 && head_size > 0 ? decode_workspace(q_heads, kv_heads, head_size) : 0;
+}
 extern "C" size_t mcop_paged_attention_chunk_workspace_bytes(int64_t tokens, int batch, int q_heads, int kv_heads, int head_size) { return 0; }
 
 extern "C" int mcop_paged_attention_decode(void* out, int64_t out_token_stride, int64_t out_head_stride, float* lse, const void* query,
@@ -210,7 +149,8 @@ extern "C" int mcop_paged_attention_decode(void* out, int64_t out_token_stride, 
              query, out, lse, query_token_stride, query_head_stride, out_token_stride, out_head_stride, seq_lens, nullptr, batch, batch, q_heads,
              head_size, scale_mode, scale, 1, window, pipe_error_ptr()};
   if (int rc = check_args(what, a, batch, dtype)) return rc;
-  return launch_rows(what, a, dtype, (cudaStream_t)stream);
+  a.c.prepare();
+  return launch_decode(a, dtype, workspace, workspace_bytes, (cudaStream_t)stream);
 }
 
 extern "C" int mcop_paged_attention_chunk(void* out, int64_t out_token_stride, int64_t out_head_stride, float* lse, const void* query,
@@ -230,5 +170,6 @@ extern "C" int mcop_paged_attention_chunk(void* out, int64_t out_token_stride, i
              query, out, lse, query_token_stride, query_head_stride, out_token_stride, out_head_stride, seq_lens, cu_seqlens_q, batch, (int)tokens,
              q_heads, head_size, scale_mode, scale, causal, window, pipe_error_ptr()};
   if (int rc = check_args(what, a, tokens, dtype)) return rc;
+  a.c.prepare();
   return launch_rows(what, a, dtype, (cudaStream_t)stream);
 }

@@ -23,6 +23,15 @@ struct PagedCache {
   int block_size;
   int64_t num_blocks;
   int kv_heads;
+  uint32_t page_mul = 0, page_shift = 0;
+
+  // The division by the block size as a multiplication: with 2^(s-1) < d <= 2^s and m = ceil(2^(31 + s) / d) < 2^32,
+  // floor(p * m / 2^(31 + s)) = floor(p / d) for every p < 2^31 (m exceeds 2^(31 + s) / d by less than 2^s / d).
+  __host__ void prepare() {
+    while ((int64_t(1) << page_shift) < block_size) ++page_shift;
+    page_mul = (uint32_t)(((uint64_t(1) << (31 + page_shift)) + block_size - 1) / block_size);
+  }
+  __device__ __forceinline__ int page_of(int p) const { return (int)(__umulhi(2u * (uint32_t)p, page_mul) >> page_shift); }
 };
 
 __device__ __forceinline__ void report(int* err, int code) {

@@ -51,15 +51,16 @@ def make_cache(total, kv_heads, D, block, kind, dtype, seed=0, poison=True, spar
 
 def attention_tolerance(ref, lse, spread, mass, reach, D, kind, dtype):
     """(for out, for lse).  out: half a step of its own rounding; each weight is rounded once to the 16-bit type that multiplies V
-    (bf16 wherever the cache is int8) - at most half a step of it per weight, so that much of sum p |v|; a logit is an fp32 sum of D
+    (f16 wherever the cache is int8) - at most half a step of it per weight, so that much of sum p |v|; a logit is an fp32 sum of D
     exact products: its error is at most (D + 4) * 2^-24 times sum |q k|, and moves each weight by twice that, relatively (the
     numerator and the total); 2^-17 covers exp2, log2 and the fp32 sums (2^-22 each, up to 32 of them in a row).  Weights far below the largest one, which is 1 or more as they are formed, leave the normal
     range: then the error is absolute, 2^-25 in f16 (half its subnormal step), 2^-126 where small numbers become 0 in fp32 and bf16,
-    times sum |v|."""
+    times sum |v|.  (With a scale per token the largest product of weight and scale takes the place of the largest weight: the
+    tests' scales lie within a factor of 3, so 2^-25 becomes at most 2^-23.)"""
     logit = (D + 4) * 2.0 ** -24 * reach
-    weight = HALF[torch.bfloat16 if kind != "float" else dtype]
+    weight = HALF[torch.float16 if kind != "float" else dtype]
     tol = HALF[dtype] * ref.abs() + (weight + 2 * logit + 2.0 ** -17)[..., None] * spread * (1 + HALF[dtype])
-    tol = tol + mass * (2.0 ** -25 if kind == "float" and dtype == torch.float16 else 2.0 ** -126)
+    tol = tol + mass * (2.0 ** -23 if kind == "token" else 2.0 ** -25 if kind == "head" or dtype == torch.float16 else 2.0 ** -126)
     tol = tol + (2.0 ** -25 if dtype == torch.float16 else 2.0 ** -134)  # half the output's own subnormal step
     return tol, logit + 2.0 ** -17 + 2.0 ** -23 * lse.abs()
 

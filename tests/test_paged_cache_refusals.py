@@ -40,10 +40,11 @@ def test_gather_refuses(change):
 
 ATTENTION = COMMON + [dict(q=None), dict(out=None), dict(lens=None), dict(tab=None), dict(mode=1), dict(mode=4), dict(dtype=0), dict(hq=12),
                       dict(hq=0), dict(q=24), dict(qt=1001), dict(oh=100), dict(tstride=-1), dict(maxb=-1), dict(maxb=1 << 28, tstride=1 << 28),
-                      dict(window=-1), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(batch=-1)]
+                      dict(window=-1), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(batch=-1), dict(bs=1 << 33),
+                      dict(bs=-16384)]
 
 
-@pytest.mark.parametrize("change", ATTENTION)
+@pytest.mark.parametrize("change", ATTENTION + [dict(ws=24, wsb=1 << 30), dict(ws=16, wsb=64)])
 def test_decode_refuses(change):
     rc, text = _call("mcop_paged_attention_decode", DECODE, **change)
     assert rc < 0 and "paged_attention_decode" in text
