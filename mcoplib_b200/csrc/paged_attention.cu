@@ -130,9 +130,12 @@ int launch_rows(const char* what, const AttnArgs& a, int dtype, cudaStream_t st)
 using namespace mcop;
 
 extern "C" size_t mcop_paged_attention_decode_workspace_bytes(int batch, int q_heads, int kv_heads, int head_size) {
-  return batch > 0 && kv_heads > 0 && q_heads > 0 && head_size > 0 ? decode_workspace(q_heads, kv_heads, head_size) : 0;
+  return batch > 0 && kv_heads > 0 && q_heads >= kv_heads && head_size > 0 ? decode_workspace(q_heads, kv_heads, head_size) : 0;
 }
-extern "C" size_t mcop_paged_attention_chunk_workspace_bytes(int64_t tokens, int batch, int q_heads, int kv_heads, int head_size) { return 0; }
+extern "C" size_t mcop_paged_attention_chunk_workspace_bytes(int64_t tokens, int batch, int q_heads, int kv_heads, int head_size) {
+  const bool any = tokens > 0 && batch > 0 && kv_heads > 0 && q_heads >= kv_heads && head_size > 0 && head_size <= kChunkHead;
+  return any ? chunk_workspace(tokens, batch, q_heads, kv_heads, head_size) : 0;
+}
 
 extern "C" int mcop_paged_attention_decode(void* out, int64_t out_token_stride, int64_t out_head_stride, float* lse, const void* query,
                                            int64_t query_token_stride, int64_t query_head_stride, const void* key_cache,
@@ -171,5 +174,6 @@ extern "C" int mcop_paged_attention_chunk(void* out, int64_t out_token_stride, i
              q_heads, head_size, scale_mode, scale, causal, window, pipe_error_ptr()};
   if (int rc = check_args(what, a, tokens, dtype)) return rc;
   a.c.prepare();
+  if (a.head_size <= kChunkHead) return launch_chunk(a, dtype, workspace, workspace_bytes, (cudaStream_t)stream);
   return launch_rows(what, a, dtype, (cudaStream_t)stream);
 }

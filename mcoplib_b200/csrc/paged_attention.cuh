@@ -32,19 +32,20 @@ struct Seq {
 };
 
 // Bounds of sequence b, checked: what the caller's tensors say is never turned into an address beyond the buffers.
-__device__ __forceinline__ Seq sequence(const AttnArgs& a, int b) {
+// REPORT: whether this call records what it finds wrong (once per launch is enough).
+template <bool REPORT = true> __device__ __forceinline__ Seq sequence(const AttnArgs& a, int b) {
   Seq s;
   s.q0 = a.cu ? a.cu[b] : b;
   const int q1 = a.cu ? a.cu[b + 1] : b + 1;
   s.qn = q1 - s.q0;
   if (s.q0 < 0 || q1 < s.q0 || q1 > a.tokens) {
-    report(a.err, MCOP_DEVERR_SEQUENCE);
+    if (REPORT) report(a.err, MCOP_DEVERR_SEQUENCE);
     s.q0 = s.qn = 0;
   }
   s.len = a.seq_lens[b];
   const int64_t room = (int64_t)a.c.max_blocks * a.c.block_size;
   if (s.len < 0 || s.len > room) {
-    report(a.err, MCOP_DEVERR_KV_INDEX);
+    if (REPORT) report(a.err, MCOP_DEVERR_KV_INDEX);
     s.len = s.len < 0 ? 0 : (int)room;
   }
   return s;
@@ -87,5 +88,10 @@ __device__ __forceinline__ float exp2_approx(float x) {
 // Decode (paged_decode.cu): one new token per sequence, head sizes up to 256.
 size_t decode_workspace(int q_heads, int kv_heads, int head_size);
 int launch_decode(const AttnArgs& a, int dtype, void* ws, size_t ws_bytes, cudaStream_t st);
+
+// Chunk (paged_chunk.cu): head sizes up to 128.
+constexpr int kChunkHead = 128;
+size_t chunk_workspace(int64_t tokens, int batch, int q_heads, int kv_heads, int head_size);
+int launch_chunk(const AttnArgs& a, int dtype, void* ws, size_t ws_bytes, cudaStream_t st);
 
 }  // namespace mcop

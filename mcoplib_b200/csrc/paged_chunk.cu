@@ -1,0 +1,892 @@
+// Chunk attention on the fifth-generation tensor cores: a run of new tokens per sequence over its cached tokens.
+//
+// The rows of a work item are (new token, query head) pairs of one sequence and one KV head, in that order: all query heads of a
+// KV head share the tiles of K and V, and a short chunk still fills a tile.  256 rows make an item: two M = 128 tiles, so that the
+// tensor cores form the logits of one tile while the other tile's softmax runs.
+//   S[128 x 128] = Q[128 x D] K^T        (both operands in shared memory, S in tensor memory)
+//   P = exp2(S * c - m)                  (a thread owns a row: no shuffles; P goes back to tensor memory over S, in 16 bits)
+//   O[128 x D]  += P[128 x 128] V        (P from tensor memory, V in shared memory as it lies: MN-major)
+// Roles (16 warps, registers dealt by setmaxnreg): 2 x 4 warps of softmax, 4 warps that bring Q, K and V into shared memory, one
+// thread that issues the MMAs.  K and V pass through a ring of 16-bit tiles of 128 tokens; rows are gathered from their pages, and int8
+// codes become bf16 (K, beside bf16 queries) or f16 on the way, exactly: their scales multiply logits and weights in fp32.  The
+// running maximum is moved (and O rescaled) only when a logit passes it by 2^8.
+//
+// Work split: the (item, 128-token tile) pairs of the whole call form one line, cut into equal ranges, one per CTA and SM; a first
+// launch of one CTA lays the line out from the lengths on the device (so a captured graph serves any), a third joins the items
+// that cross a border, in a fixed order.
+//
+// Bound: per pair of 256 x 128 logits 2 x 256 x 128 x D x 2 flops of MMA (2048 cycles at D = 128) and 32,768 exponentials (2048
+// cycles of the SM's 16 per cycle): the two are equal, and everything else has to hide behind them.
+#include "paged_attention.cuh"
+#include "tcgen05.cuh"
+
+namespace mcop {
+namespace {
+
+constexpr int kRows = 256, kTile = 128, kThreads = 512;
+// Fewer tiles than this per CTA are not worth a partial result of their own.
+constexpr int kMinTiles = 2;
+constexpr uint32_t kSpin = 1u << 20;  // tries of a wait
+constexpr int kWaitSoftmax = 8, kWaitLoad = 9, kWaitMma = 10;  // codes of the error word
+
+// The line of work, in the workspace: prefix[i] = 128-token tiles (of one KV head) in front of query tile i.
+struct PlanTile {
+  int b, t, rows, pad;  // sequence, tile of it, rows of the tile that are there
+};
+struct Plan {
+  int tiles, pad[3];
+};
+struct Rec {
+  int b, t, head, count;
+};
+struct Layout {  // of the workspace
+  Plan* plan;
+  int64_t* prefix;      // [max_tiles + 1]
+  PlanTile* tile;       // [max_tiles]
+  int64_t* seq_tiles;   // [batch + 1]
+  Rec* recs;            // [ctas]
+  float* parts;         // [2 * ctas] slots: O [256][DP], then (maximum, sum) [256][2]
+};
+__host__ __device__ inline int64_t max_tiles(int64_t tokens, int batch, int group) { return tokens * group / kRows + batch; }
+__host__ __device__ inline size_t up16(size_t n) { return (n + 15) / 16 * 16; }
+__host__ inline size_t layout(char* ws, int64_t tokens, int batch, int group, int dp, int ctas, Layout* l) {
+  const int64_t mt = max_tiles(tokens, batch, group);
+  size_t at = 0;
+  auto take = [&](size_t bytes) { const size_t was = at; at += up16(bytes); return ws + was; };
+  Layout x;
+  x.plan = (Plan*)take(sizeof(Plan));
+  x.prefix = (int64_t*)take((mt + 1) * 8);
+  x.tile = (PlanTile*)take(mt * sizeof(PlanTile));
+  x.seq_tiles = (int64_t*)take((batch + 1) * 8);
+  x.recs = (Rec*)take(ctas * sizeof(Rec));
+  x.parts = (float*)take((size_t)ctas * 2 * kRows * (dp + 2) * 4);
+  if (l) *l = x;
+  return at;
+}
+
+// Tiles [first, first + n) of 128 tokens that the rows of query tile t of a sequence see between them; tokens [lo, hi).
+struct Reach {
+  int first, n, lo, hi;
+};
+__device__ __forceinline__ Reach reach(const AttnArgs& a, const Seq& s, int t, int group) {
+  const int i0 = t * kRows / group, i1 = min(s.qn - 1, (t * kRows + kRows - 1) / group);
+  Reach r;
+  int other;
+  span(a, s, i0, r.lo, other);
+  span(a, s, i1, other, r.hi);
+  r.lo = min(r.lo, r.hi);
+  r.first = r.lo / kTile;
+  r.n = max(1, (r.hi + kTile - 1) / kTile - r.first);
+  return r;
+}
+
+__global__ void __launch_bounds__(1024) chunk_plan_kernel(AttnArgs a, Layout w, int64_t limit) {
+  pdl_launch_dependents();
+  pdl_wait();
+  __shared__ int64_t sums[33];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = a.q_heads / a.c.kv_heads;
+  auto scan = [&](int64_t v) {  // inclusive over the CTA; sums[32] = total
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    if (lane == 31) sums[warp] = v;
+    __syncthreads();
+    if (warp == 0) {
+      int64_t u = sums[lane];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t x = __shfl_up_sync(0xffffffffu, u, o);
+        if (lane >= o) u += x;
+      }
+      sums[lane] = u;
+      if (lane == 31) sums[32] = u;
+    }
+    __syncthreads();
+    if (warp) v += sums[warp - 1];
+    const int64_t total = sums[32];
+    __syncthreads();
+    return make_longlong2(v, total);
+  };
+  auto count = [&](int b) { return (int64_t)((int64_t)sequence(a, b).qn * G + kRows - 1) / kRows; };
+  int64_t base = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 1024) {
+    const int b = b0 + tid;
+    const int64_t n = b < a.batch ? count(b) : 0;
+    const longlong2 s = scan(n);
+    if (b < a.batch) w.seq_tiles[b] = base + s.x - n;
+    base += s.y;
+  }
+  // sequences that overlap (reported as descending bounds) could add up to more than there is room for
+  const int64_t tiles = min(base, limit);
+  if (tid == 0) {
+    w.seq_tiles[a.batch] = base;
+    w.plan->tiles = (int)tiles;
+  }
+  __syncthreads();
+  int64_t front = 0;
+  for (int64_t i0 = 0; i0 < tiles; i0 += 1024) {
+    const int64_t i = i0 + tid;
+    int64_t n = 0;
+    if (i < tiles) {
+      int lo = 0, hi = a.batch;  // seq_tiles[lo] <= i < seq_tiles[hi]
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (w.seq_tiles[mid] <= i) lo = mid;
+        else hi = mid;
+      }
+      const int t = (int)(i - w.seq_tiles[lo]);
+      const Seq s = sequence<false>(a, lo);
+      w.tile[i] = PlanTile{lo, t, (int)min((int64_t)kRows, (int64_t)s.qn * G - (int64_t)t * kRows), 0};
+      n = reach(a, s, t, G).n;
+    }
+    const longlong2 s = scan(n);
+    if (i < tiles) w.prefix[i] = front + s.x - n;
+    front += s.y;
+  }
+  if (tid == 0) w.prefix[tiles] = front;
+}
+
+template <typename T, int MODE, int DP> struct Cfg {
+  static constexpr bool I8 = MODE != kScaleNone;
+  static constexpr int HALF = kTile * 128;               // 64 columns of 128 rows, 128-byte swizzle
+  static constexpr int TILE = HALF * (DP / 64);          // a 16-bit tile of 128 rows
+  static constexpr int ST = DP == 128 ? 4 : 8;
+  static constexpr int SMEM = 2 * TILE + ST * TILE + 1024;
+  static constexpr int PIECES = DP / 8;                  // 16-byte pieces of a row in shared memory
+};
+
+// A piece of work of a CTA: query tile `tile` of the plan against tiles [k0, k1) of the n of its reach, for one KV head.
+struct Work {
+  int tile, head, k0, k1, n;
+};
+struct WorkLine {
+  int left, tile, head, k;  // tiles of 128 tokens still to do; where the next piece begins
+  __device__ __forceinline__ static int64_t total(const Layout& w, int kv_heads) { return w.plan->tiles ? w.prefix[w.plan->tiles] * kv_heads : 0; }
+  __device__ __forceinline__ static int64_t per(int64_t total) { return max((int64_t)kMinTiles, (total + gridDim.x - 1) / gridDim.x); }
+  __device__ __forceinline__ void start(const Layout& w, int kv_heads) {
+    const int64_t all = total(w, kv_heads), share = per(all), u = share * blockIdx.x;
+    left = (int)max((int64_t)0, min(all - u, share));
+    if (left == 0) return;
+    int lo = 0, hi = w.plan->tiles;  // prefix[lo] * kv_heads <= u < prefix[hi] * kv_heads
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (w.prefix[mid] * kv_heads <= u) lo = mid;
+      else hi = mid;
+    }
+    tile = lo;
+    const int64_t off = u - w.prefix[lo] * kv_heads, n = w.prefix[lo + 1] - w.prefix[lo];
+    head = (int)(off / n);
+    k = (int)(off - head * n);
+  }
+  __device__ __forceinline__ bool next(const Layout& w, int kv_heads, Work& x) {
+    if (left <= 0) return false;
+    x.tile = tile;
+    x.head = head;
+    x.n = (int)(w.prefix[tile + 1] - w.prefix[tile]);
+    x.k0 = k;
+    x.k1 = min(x.n, k + left);
+    left -= x.k1 - x.k0;
+    k = 0;
+    if (++head == kv_heads) { head = 0; ++tile; }
+    return true;
+  }
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void sts_u4(uint32_t dst, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void async_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (ElemTraits<T>::code == MCOP_BF16) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&h);
+  } else {
+    __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&h);
+  }
+}
+// Two codes (bytes 0 and 2 of x) as a pair of T, exactly: 128 + seven bits minus 128 or 256 in bf16, 1024 + (code + 128) in f16.
+template <typename T> __device__ __forceinline__ uint32_t codes2(uint32_t x) {
+  if constexpr (ElemTraits<T>::code == MCOP_BF16) {
+    const uint32_t lo = (x & 0x007f007fu) | 0x43004300u, hi = (x & 0x00800080u) | 0x43004300u;
+    __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&lo), *reinterpret_cast<const __nv_bfloat162*>(&hi));
+    return *reinterpret_cast<uint32_t*>(&r);
+  } else {
+    const uint32_t u = (x & 0x00ff00ffu) ^ 0x64806480u, off = 0x64806480u;
+    __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&u), *reinterpret_cast<const __half2*>(&off));
+    return *reinterpret_cast<uint32_t*>(&r);
+  }
+}
+// Whether one of the eight 16-bit floats is a NaN or an infinity; `clean` gets them with those replaced by 0.
+template <typename T> __device__ __forceinline__ bool not_finite(uint4& u) {
+  constexpr uint32_t E = ElemTraits<T>::code == MCOP_BF16 ? 0x7f80u : 0x7c00u;
+  bool bad = false;
+  uint32_t* w = reinterpret_cast<uint32_t*>(&u);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if ((w[i] & E) == E) { bad = true; w[i] &= 0xffff0000u; }
+    if ((w[i] >> 16 & E) == E) { bad = true; w[i] &= 0x0000ffffu; }
+  }
+  return bad;
+}
+
+template <int ST> struct Bars {
+  uint64_t full[ST], empty[ST], q_full, q_empty, s_full[2], p_full[2], o_full[2], o_empty[2], info_full[ST], drain;
+};
+struct Ring {
+  int s = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void advance(int n) {
+    if (++s == n) { s = 0; phase ^= 1u; }
+  }
+};
+// What the softmax has to know of a tile's tokens beside the logits.
+struct alignas(16) TileInfo {
+  float ks[kTile], vs[kTile];  // kScaleToken: K scale times the logit factor, V scale times 2^-e
+  uint32_t here[4];            // which tokens are there (their page is in the cache)
+  int all, e;                  // all of those inside the reach are; e of the V scales
+};
+struct TileBits {
+  uint32_t here[4];
+  int all, e;
+};
+
+template <typename T, int MODE, int DP>
+__global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w) {
+  using C = Cfg<T, MODE, DP>;
+  using VT = typename std::conditional<C::I8, __half, T>::type;  // type of P and V
+  using Info = typename std::conditional<MODE == kScaleToken, TileInfo, TileBits>::type;
+  constexpr int ST = C::ST;
+  extern __shared__ __align__(16) unsigned char raw[];
+  __shared__ Bars<ST> bars;
+  __shared__ Info info[ST];
+  __shared__ uint32_t tmem_at;
+  __shared__ uint32_t row_at[2][kTile];   // cached rows of a tile, in units of 16 bytes
+  __shared__ uint32_t q_at[kRows];        // rows of a query tile, in units of 8 elements (0xffffffff: none)
+  __shared__ float vmax[2][4];
+  __shared__ int poison[8];               // items whose masked tiles hold a NaN or an infinity in V
+  pdl_launch_dependents();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, group = warp >> 2;
+  unsigned char* const smem = raw + (1024 - (smem_addr(raw) & 1023)) % 1024;
+  unsigned char* const q_smem = smem;
+  unsigned char* const ring = smem + 2 * C::TILE;
+  if (tid == 0) {
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(&bars.full[i], 4);
+      mbar_init(&bars.empty[i], 1);
+      mbar_init(&bars.info_full[i], 4);
+    }
+    mbar_init(&bars.q_full, 4);
+    mbar_init(&bars.q_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars.s_full[i], 1);
+      mbar_init(&bars.p_full[i], 4);
+      mbar_init(&bars.o_full[i], 1);
+      mbar_init(&bars.o_empty[i], 4);
+    }
+    mbar_init(&bars.drain, 1);
+    mbar_init_fence();
+  }
+  if (warp == 12) tmem_alloc_all(&tmem_at);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_wait();
+  const uint32_t tmem = tmem_at;
+  const int G = a.q_heads / a.c.kv_heads;
+  WorkLine line;
+  Work x;
+  line.start(w, a.c.kv_heads);
+  if (tid == 0) w.recs[blockIdx.x].count = 0;
+
+  if (group < 2) {
+    // ------------------------------------------------------------------------------------------ softmax of tile `group`
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    const int r = tid & 127;  // row of the tile
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+    const uint32_t s_addr = tmem + lanes + group * 128, o_addr = tmem + lanes + 256 + group * DP;
+    Ring inf;
+    uint32_t s_phase = 0, o_phase = 0;
+    int item = 0;
+    bool ok = true;
+    while (ok && line.next(w, a.c.kv_heads, x)) {
+      const PlanTile pt = w.tile[x.tile];
+      const bool idle = group == 1 && pt.rows <= 128;
+      const int row = group * 128 + r;
+      const bool mine = row < pt.rows;
+      const int flat = pt.t * kRows + row, token = flat / G, head = x.head * G + flat - token * G;
+      int lo = 0, hi = INT_MAX, first, q0;
+      {
+        const Seq s = sequence<false>(a, pt.b);
+        first = reach(a, s, pt.t, G).first;
+        q0 = s.q0;
+        if (mine) span(a, s, token, lo, hi);
+      }
+      float c = a.scale * kLog2e;
+      if (MODE == kScaleHead) c *= a.c.k_scale[x.head];
+      float m = -INFINITY, l = 0.f;
+      int e = -1000;
+      if (idle) {  // no rows: keep in step with the item
+        if (!(ok = mbar_wait_bounded(&bars.o_full[group], o_phase, a.err, kWaitSoftmax, kSpin))) break;
+        o_phase ^= 1;
+        for (int k = x.k0; k < x.k1; ++k) inf.advance(ST);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.o_empty[group]);
+        ++item;
+        continue;
+      }
+      for (int k = x.k0; k < x.k1 && ok; ++k) {
+        const Info& in = info[inf.s];
+        if (!(ok = mbar_wait_bounded(&bars.info_full[inf.s], inf.phase, a.err, kWaitSoftmax, kSpin))) break;
+        inf.advance(ST);
+        if (!(ok = mbar_wait_bounded(&bars.s_full[group], s_phase, a.err, kWaitSoftmax, kSpin))) break;
+        s_phase ^= 1;
+        tc_fence_after();
+        float s[128];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tmem_ld32(s_addr + 32 * i, s + 32 * i);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tmem_loaded32(s + 32 * i);
+        // logits in log2 units
+#pragma unroll
+        for (int i = 0; i < 128; i += 4) {
+          if constexpr (MODE == kScaleToken) {
+            const float4 f = *reinterpret_cast<const float4*>(&in.ks[i]);
+            const float2 p = __fmul2_rn(make_float2(s[i], s[i + 1]), make_float2(f.x, f.y)), q = __fmul2_rn(make_float2(s[i + 2], s[i + 3]), make_float2(f.z, f.w));
+            s[i] = p.x; s[i + 1] = p.y; s[i + 2] = q.x; s[i + 3] = q.y;
+          } else {
+            const float2 p = __fmul2_rn(make_float2(s[i], s[i + 1]), make_float2(c, c)), q = __fmul2_rn(make_float2(s[i + 2], s[i + 3]), make_float2(c, c));
+            s[i] = p.x; s[i + 1] = p.y; s[i + 2] = q.x; s[i + 3] = q.y;
+          }
+        }
+        const int base = (first + k) * kTile;
+        const bool masked = __any_sync(0xffffffffu, base < lo || base + kTile > hi) || !in.all;
+        if (masked) {
+          const int from = max(0, min(kTile, lo - base)), to = hi - base;  // columns [from, to) are seen
+#pragma unroll
+          for (int i = 0; i < 128; ++i)
+            if (i < from || i >= to || !(in.here[i / 32] >> (i % 32) & 1)) s[i] = -INFINITY;
+        }
+        float top = fmaxf(s[0], s[1]);
+#pragma unroll
+        for (int i = 2; i < 128; i += 2) asm("max.f32 %0, %0, %1, %2;" : "+f"(top) : "f"(s[i]), "f"(s[i + 1]));
+        const bool grown = top > m + kMaxSlack;
+        const int e_new = in.e;
+        const bool moved = MODE == kScaleToken && e_new != e;
+        if (__any_sync(0xffffffffu, grown) || moved) {
+          const float to = grown ? top : m;
+          float keep = m == -INFINITY ? 0.f : exp2_approx(m - to);
+          m = to;
+          l *= keep;
+          if (moved) {
+            keep *= exp2_approx((float)max(-120, e - e_new));
+            e = e_new;
+          }
+          if (k > x.k0) {
+            // (S of this tile was issued behind the previous tile's P V: that product is complete)
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i) {
+              float o[32];
+              tmem_ld32(o_addr + 32 * i, o);
+              tmem_wait_ld();
+              tmem_loaded32(o);
+#pragma unroll
+              for (int d = 0; d < 32; ++d) o[d] *= keep;
+              tmem_st32(o_addr + 32 * i, o);
+            }
+          }
+        }
+        const float safe = m == -INFINITY ? 0.f : m;
+        float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t p[16];
+#pragma unroll
+          for (int d = 0; d < 16; d += 2) {
+            float2 u = make_float2(s[32 * i + 2 * d], s[32 * i + 2 * d + 1]), v = make_float2(s[32 * i + 2 * d + 2], s[32 * i + 2 * d + 3]);
+            u = __fadd2_rn(u, make_float2(-safe, -safe));
+            v = __fadd2_rn(v, make_float2(-safe, -safe));
+            u.x = exp2_approx(u.x); u.y = exp2_approx(u.y);
+            v.x = exp2_approx(v.x); v.y = exp2_approx(v.y);
+            sum0 = __fadd2_rn(sum0, u);
+            sum1 = __fadd2_rn(sum1, v);
+            if constexpr (MODE == kScaleToken) {
+              const float4 f = *reinterpret_cast<const float4*>(&in.vs[32 * i + 2 * d]);
+              if (masked) {  // a scale that is not finite reaches only the rows that see its token
+                u.x = u.x == 0.f ? 0.f : u.x * f.x; u.y = u.y == 0.f ? 0.f : u.y * f.y;
+                v.x = v.x == 0.f ? 0.f : v.x * f.z; v.y = v.y == 0.f ? 0.f : v.y * f.w;
+              } else {
+                u = __fmul2_rn(u, make_float2(f.x, f.y));
+                v = __fmul2_rn(v, make_float2(f.z, f.w));
+              }
+            }
+            p[d] = pack2<VT>(u.x, u.y);
+            p[d + 1] = pack2<VT>(v.x, v.y);
+          }
+          tmem_st16(s_addr + 16 * i, p);
+        }
+        l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.p_full[group]);
+      }
+      if (ok) {
+        // O of the item
+        if (!(ok = mbar_wait_bounded(&bars.o_full[group], o_phase, a.err, kWaitSoftmax, kSpin))) break;
+        o_phase ^= 1;
+        tc_fence_after();
+        const bool whole = x.k1 - x.k0 == x.n;
+        float f = 1.f;
+        if (MODE == kScaleToken) f = exp2_approx((float)e);
+        if (MODE == kScaleHead) f = a.c.v_scale[x.head];
+        const float norm = whole ? (l == 0.f ? 0.f : f / l) : f;
+        float* part = w.parts + (int64_t)(2 * blockIdx.x + (x.k0 == 0 ? 1 : 0)) * (kRows * (DP + 2));
+        T* out = static_cast<T*>(a.out) + (int64_t)(q0 + token) * a.o_token + (int64_t)head * a.o_head;
+        const bool sick = !C::I8 && *(volatile int*)&poison[item & 7];
+#pragma unroll 1
+        for (int i = 0; i < DP / 32; ++i) {
+          float o[32];
+          __syncwarp();
+          tmem_ld32(o_addr + 32 * i, o);
+          tmem_wait_ld();
+          tmem_loaded32(o);
+          if (i == DP / 32 - 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.o_empty[group]);
+          }
+          if constexpr (!C::I8) {
+            if (sick && mine) {  // the masked tiles were added up without their NaNs and infinities: add those that this row sees
+              for (int k = x.k0; k < x.k1; ++k) {
+                const int base = (first + k) * kTile;
+                for (int j = max(lo, base); j < min(hi, base + kTile); ++j) {
+                  const int slot = slot_of(a, pt.b, j);
+                  if (slot < 0) continue;
+                  const T* v = static_cast<const T*>(a.c.v) + row_of(a.c, slot, x.head) + 32 * i;
+                  for (int d = 0; d < 32 && 32 * i + d < a.head_size; ++d) {
+                    const float y = ElemTraits<T>::to_float(v[d]);
+                    if (!(fabsf(y) <= FLT_MAX)) {
+#pragma unroll
+                      for (int z = 0; z < 32; ++z)
+                        if (z == d) o[z] += y;
+                    }
+                  }
+                }
+              }
+            }
+          }
+#pragma unroll
+          for (int d = 0; d < 32; ++d) o[d] *= norm;
+          if (!mine) {
+          } else if (whole) {
+#pragma unroll
+            for (int d = 0; d < 32; d += 8)
+              if (32 * i + d < a.head_size)
+                *reinterpret_cast<uint4*>(out + 32 * i + d) = make_uint4(pack2<T>(o[d], o[d + 1]), pack2<T>(o[d + 2], o[d + 3]), pack2<T>(o[d + 4], o[d + 5]),
+                                                                         pack2<T>(o[d + 6], o[d + 7]));
+          } else {
+#pragma unroll
+            for (int d = 0; d < 32; d += 4) *reinterpret_cast<float4*>(part + row * DP + 32 * i + d) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
+          }
+        }
+        if (mine) {
+          if (!whole) *reinterpret_cast<float2*>(part + kRows * DP + 2 * row) = make_float2(m, l);
+          else if (a.lse) a.lse[(int64_t)(q0 + token) * a.q_heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+        }
+      }
+      if (tid == 0 && line.left == 0 && x.k0 == 0 && x.k1 < x.n) {  // the item that begins here and goes on in the next CTA
+        const int64_t share = WorkLine::per(WorkLine::total(w, a.c.kv_heads)), last = share * (blockIdx.x + 1) - 1 + (x.n - x.k1);
+        w.recs[blockIdx.x] = Rec{pt.b, pt.t, x.head, (int)(last / share - blockIdx.x) + 1};
+      }
+      ++item;
+    }
+  } else if (group == 2) {
+    // ------------------------------------------------------------------------------------------ Q, K and V into shared memory
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    const int lt = tid & 127, lwarp = warp & 3;
+    const int row_pieces = a.head_size * (C::I8 ? 1 : 2) / 16;  // 16-byte pieces of a cached row
+    const uint32_t block16 = (uint32_t)(a.c.block_stride * (C::I8 ? 1 : 2) / 16), page16 = (uint32_t)(a.c.page_stride * (C::I8 ? 1 : 2) / 16),
+                   head16 = (uint32_t)(a.c.head_stride * (C::I8 ? 1 : 2) / 16);
+    const char* kbase = static_cast<const char*>(a.c.k);
+    const char* vbase = static_cast<const char*>(a.c.v);
+    auto sync = [&]() { asm volatile("bar.sync 1, 128;" ::: "memory"); };
+    auto sync_and = [&](bool v) {
+      uint32_t r;
+      asm volatile(
+          "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+          : "=r"(r)
+          : "r"((uint32_t)v)
+          : "memory");
+      return r != 0;
+    };
+    Ring st, done, inf;       // stage to fill next, stage to hand over next, tile information to fill next
+    uint32_t q_phase = 0;
+    int pending = 0;          // copies issued and not handed over (float caches)
+    uint32_t with_q = 0, scan_v = 0;  // one bit per pending copy, the oldest in bit pending - 1: Q came with it; V of a masked tile
+    uint32_t scan_item = 0;
+    bool ok = true;
+    int item = 0, buf = 0;
+
+    // hands over the oldest pending copy
+    auto hand_over = [&]() {
+      const uint32_t bit = 1u << (pending - 1);
+      if constexpr (!C::I8) {
+        if (scan_v & bit) {  // a NaN or an infinity times the weight 0 of a row that does not see it would be NaN
+          const int c = lt % C::PIECES;
+          bool bad = false;
+          for (int row = lt / C::PIECES; row < kTile; row += 128 / C::PIECES) {
+            uint4* p = reinterpret_cast<uint4*>(ring + done.s * C::TILE + (c / 8) * C::HALF + row * 128 + ((c % 8) ^ (row % 8)) * 16);
+            uint4 u = *p;
+            if (not_finite<T>(u)) { *p = u; bad = true; }
+          }
+          if (bad) *(volatile int*)&poison[scan_item >> (4 * (pending - 1)) & 7] = 1;
+        }
+      }
+      async_proxy_fence();
+      __syncwarp();
+      if (lane == 0) {
+        if (with_q & bit) mbar_arrive(&bars.q_full);
+        mbar_arrive(&bars.full[done.s]);
+      }
+      with_q &= ~bit;
+      scan_v &= ~bit;
+      --pending;
+      done.advance(ST);
+    };
+    constexpr int kDepth = 3;  // copies in flight while the next one is issued
+    auto committed = [&](bool q, bool scan) {
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      with_q = with_q << 1 | (q ? 1u : 0u);
+      scan_v = scan_v << 1 | (scan ? 1u : 0u);
+      scan_item = scan_item << 4 | (uint32_t)(item & 7);
+      ++pending;
+      if (pending > kDepth) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kDepth) : "memory");
+        hand_over();
+      }
+    };
+
+    // Waits for a barrier; copies that have arrived meanwhile are handed over first, since what frees the barrier may need them.
+    auto acquire = [&](uint64_t* bar, uint32_t phase) {
+      while (pending > 0 && !__any_sync(0xffffffffu, mbar_try_wait(bar, phase))) {
+        switch (pending) {
+          case 1: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
+          case 2: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
+          default: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
+        }
+        hand_over();
+      }
+      return mbar_wait_bounded(bar, phase, a.err, kWaitLoad, kSpin);
+    };
+
+    while (ok && line.next(w, a.c.kv_heads, x)) {
+      if (lt == 0) *(volatile int*)&poison[item & 7] = 0;
+      // rows of Q
+      const PlanTile pt = w.tile[x.tile];
+      const Seq seq = sequence<false>(a, pt.b);
+      const Reach reached = reach(a, seq, pt.t, G);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = lt + 128 * i, flat = pt.t * kRows + row, token = flat / G;
+        q_at[row] = row < pt.rows ? (uint32_t)(((int64_t)(seq.q0 + token) * a.q_token + (int64_t)(x.head * G + flat - token * G) * a.q_head) / 8) : 0xffffffffu;
+      }
+      if (item > 0) {
+        if (!(ok = acquire(&bars.q_empty, q_phase))) break;
+        q_phase ^= 1;
+      }
+      sync();
+      {
+        const int c = lt % C::PIECES;
+        for (int row = lt / C::PIECES; row < (pt.rows + 127) / 128 * 128; row += 128 / C::PIECES) {
+          const uint32_t at = q_at[row];
+          const bool live = at != 0xffffffffu && c * 8 < a.head_size;
+          cp_async16(smem_addr(q_smem + (row / 128) * C::TILE + (c / 8) * C::HALF + (row % 128) * 128 + ((c % 8) ^ (row % 8)) * 16),
+                     live ? static_cast<const T*>(a.q) + (int64_t)at * 8 + c * 8 : static_cast<const T*>(a.q), live);
+        }
+      }
+      // tokens that all rows of the item see: tiles inside need no care for what a row must not see
+      int all_lo, all_hi, other;
+      span(a, seq, (pt.t * kRows + pt.rows - 1) / G, all_lo, other);
+      span(a, seq, pt.t * kRows / G, other, all_hi);
+      int e = -1000;
+      // page of token `lt` of a tile, fetched a tile ahead
+      int block = -1, off = -1;
+      auto look_up = [&](int k) {
+        off = -1;
+        if (k >= x.k1) return;
+        const int pos = (reached.first + k) * kTile + lt;
+        if (pos < reached.lo || pos >= reached.hi) return;
+        const int page = a.c.page_of(pos);
+        off = pos - page * a.c.block_size;
+        block = a.c.tables[pt.b * a.c.table_stride + page];
+      };
+      look_up(x.k0);
+      for (int k = x.k0; k < x.k1 && ok; ++k) {
+        // --- where the tile's rows are, and what the softmax needs to know of them
+        const bool known = (uint32_t)block < (uint32_t)a.c.num_blocks, here = off >= 0 && known;
+        if (off >= 0 && !known) report(a.err, MCOP_DEVERR_SLOT);
+        row_at[buf][lt] = here ? (uint32_t)block * block16 + (uint32_t)off * page16 + (uint32_t)x.head * head16 : 0xffffffffu;
+        Info& in = info[inf.s];
+        const uint32_t word = __ballot_sync(0xffffffffu, here);
+        float ks = 0.f, vs = 0.f;
+        if constexpr (MODE == kScaleToken) {
+          const int64_t at = here ? ((int64_t)block * a.c.block_size + off) * a.c.kv_heads + x.head : 0;
+          if (here) { ks = a.c.k_scale[at]; vs = a.c.v_scale[at]; }
+          const float top = warp_max(fabsf(vs) <= FLT_MAX ? fabsf(vs) : 0.f);
+          if (lane == 0) vmax[buf][lwarp] = top;
+        }
+        const bool sound = sync_and(off < 0 || known);
+        if constexpr (MODE == kScaleToken) {
+          const float top = fmaxf(fmaxf(vmax[buf][0], vmax[buf][1]), fmaxf(vmax[buf][2], vmax[buf][3]));
+          // 2^e >= the tile's largest scale; moved only upwards and by more than 2^6, so that weight times scale stays below
+          // 2^14 (f16 ends at 2^16) and O is rescaled rarely
+          const int need = max((int)(__float_as_uint(top) >> 23) - 126, -100);
+          if (need > e + 6) e = need;
+          in.ks[lt] = ks * (a.scale * kLog2e);
+          in.vs[lt] = vs * exp2_approx((float)-e);
+        }
+        if (lane == 0) {
+          in.here[lwarp] = word;
+          if (lwarp == 0) { in.all = sound ? 1 : 0; in.e = e; }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.info_full[inf.s]);
+        inf.advance(ST);
+        look_up(k + 1);
+        // --- K, then V
+        const int base = (reached.first + k) * kTile;
+        const bool scan = base < all_lo || base + kTile > all_hi;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          const char* src = kv ? vbase : kbase;
+          if constexpr (!C::I8) {
+            if (!(ok = acquire(&bars.empty[st.s], st.phase ^ 1))) break;
+            unsigned char* dst = ring + st.s * C::TILE;
+            const int c = lt % C::PIECES;
+#pragma unroll
+            for (int i = 0; i < kTile * C::PIECES / 128; ++i) {
+              const int row = lt / C::PIECES + i * (128 / C::PIECES);
+              const uint32_t at = row_at[buf][row];
+              const bool live = at != 0xffffffffu && c < row_pieces;
+              cp_async16(smem_addr(dst + (c / 8) * C::HALF + row * 128 + ((c % 8) ^ (row % 8)) * 16), live ? src + (uint64_t)at * 16 + c * 16 : src, live);
+            }
+            st.advance(ST);
+            committed(kv == 0 && k == x.k0, kv == 1 && scan);
+          } else {
+            constexpr int IP = DP / 16, N = kTile * IP / 128;  // 16-byte pieces of an int8 row; pieces per thread
+            const int c = lt % IP;
+            uint4 u[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+              const uint32_t at = row_at[buf][lt / IP + i * (128 / IP)];
+              u[i] = make_uint4(0, 0, 0, 0);
+              if (at != 0xffffffffu && c < row_pieces) u[i] = ld_nc_u4(src + (uint64_t)at * 16 + c * 16);
+            }
+            if (!(ok = mbar_wait_bounded(&bars.empty[st.s], st.phase ^ 1, a.err, kWaitLoad, kSpin))) break;
+            unsigned char* dst = ring + st.s * C::TILE;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+              const int row = lt / IP + i * (128 / IP);
+              const uint32_t wd[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+              uint32_t y[8];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const uint32_t p = __byte_perm(wd[j], 0, 0x4140), q = __byte_perm(wd[j], 0, 0x4342);
+                y[2 * j] = kv ? codes2<VT>(p) : codes2<T>(p);
+                y[2 * j + 1] = kv ? codes2<VT>(q) : codes2<T>(q);
+              }
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int piece = 2 * c + h;
+                sts_u4(smem_addr(dst + (piece / 8) * C::HALF + row * 128 + ((piece % 8) ^ (row % 8)) * 16), y[4 * h], y[4 * h + 1], y[4 * h + 2], y[4 * h + 3]);
+              }
+            }
+            if (kv == 0 && k == x.k0) asm volatile("cp.async.wait_all;" ::: "memory");
+            async_proxy_fence();
+            __syncwarp();
+            if (lane == 0) {
+              if (kv == 0 && k == x.k0) mbar_arrive(&bars.q_full);
+              mbar_arrive(&bars.full[st.s]);
+            }
+            st.advance(ST);
+          }
+        }
+        buf ^= 1;
+      }
+      ++item;
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if constexpr (!C::I8) {
+      while (pending > 0) hand_over();
+    }
+  } else {
+    // ------------------------------------------------------------------------------------------ the MMAs
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 12 && lane == 0) {
+      constexpr uint32_t QK = f16_idesc(ElemTraits<T>::code == MCOP_BF16, 128, kTile, false);
+      constexpr uint32_t PV = f16_idesc(ElemTraits<VT>::code == MCOP_BF16, 128, DP, true);
+      const uint32_t q_addr = smem_addr(q_smem), ring_addr = smem_addr(ring);
+      Ring st;
+      uint32_t q_phase = 0, p_phase[2] = {0, 0}, oe_phase[2] = {1, 1};
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t phase) {
+        ok = ok && mbar_wait_bounded(bar, phase, a.err, kWaitMma, kSpin);
+        tc_fence_after();
+        return ok;
+      };
+      auto logits = [&](int tile, int stage) {
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+          const uint32_t at = (i / 4) * C::HALF + (i % 4) * 32;
+          tc_mma_ss(tmem + tile * 128, smem_desc(q_addr + tile * C::TILE + at, 16, 1024), smem_desc(ring_addr + stage * C::TILE + at, 16, 1024), QK, i > 0);
+        }
+        tc_commit(&bars.s_full[tile]);
+      };
+      auto values = [&](int tile, int stage, bool more) {
+#pragma unroll
+        for (int i = 0; i < kTile / 16; ++i)
+          tc_mma_ts(tmem + 256 + tile * DP, tmem + tile * 128 + 8 * i, smem_desc(ring_addr + stage * C::TILE + i * 2048, C::HALF, 1024), PV, more || i > 0);
+      };
+      while (ok && line.next(w, a.c.kv_heads, x)) {
+        const int two = w.tile[x.tile].rows > 128 ? 2 : 1;
+        if (!wait(&bars.q_full, q_phase)) break;
+        q_phase ^= 1;
+        if (!wait(&bars.full[st.s], st.phase)) break;
+        for (int t = 0; t < two; ++t) logits(t, st.s);
+        tc_commit(&bars.empty[st.s]);
+        if (x.k1 - x.k0 == 1) tc_commit(&bars.q_empty);
+        st.advance(ST);
+        for (int k = x.k0; k < x.k1 && ok; ++k) {
+          Ring v = st;
+          st.advance(ST);
+          const bool last = k + 1 == x.k1;
+          if (!wait(&bars.full[v.s], v.phase)) break;
+          for (int t = 0; t < two && ok; ++t) {
+            if (!wait(&bars.p_full[t], p_phase[t])) break;
+            p_phase[t] ^= 1;
+            if (k == x.k0) {  // the item before has left O
+              if (!wait(&bars.o_empty[t], oe_phase[t])) break;
+              oe_phase[t] ^= 1;
+            }
+            values(t, v.s, k > x.k0);
+            if (last) tc_commit(&bars.o_full[t]);
+            else {
+              if (t == 0 && !wait(&bars.full[st.s], st.phase)) break;
+              logits(t, st.s);
+            }
+          }
+          if (!ok) break;
+          if (last && two == 1) {  // the other tile has no rows in this item: its warps only hear that it is over
+            if (!wait(&bars.o_empty[1], oe_phase[1])) break;
+            oe_phase[1] ^= 1;
+            tc_commit(&bars.o_full[1]);
+          }
+          tc_commit(&bars.empty[v.s]);
+          if (!last) {
+            tc_commit(&bars.empty[st.s]);
+            if (k + 2 == x.k1) tc_commit(&bars.q_empty);
+            st.advance(ST);
+          }
+        }
+      }
+      // whatever is still running must not outlive the CTA's tensor memory
+      tc_commit(&bars.drain);
+      (void)mbar_wait_bounded(&bars.drain, 0, a.err, kWaitMma, kSpin);
+    }
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 12) tmem_free_all(tmem);
+}
+
+// Joins the partial results of the items that cross CTA borders: CTA c of the kernel above holds the first part of at most one such
+// item, the CTAs behind it one part each.  blockIdx.y: 32 rows; a thread takes four elements of one row at a time.
+template <typename T, int DP> __global__ void __launch_bounds__(256) chunk_join_kernel(AttnArgs a, Layout w) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const Rec rec = w.recs[blockIdx.x];
+  if (rec.count == 0) return;
+  const int G = a.q_heads / a.c.kv_heads, d = threadIdx.x % (DP / 4) * 4;
+  const Seq s = sequence(a, rec.b);
+  auto part = [&](int i) { return w.parts + (int64_t)(i == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + i)) * (kRows * (DP + 2)); };
+  for (int i = threadIdx.x / (DP / 4); i < 32; i += 1024 / DP) {
+    const int row = blockIdx.y * 32 + i, flat = rec.t * kRows + row, token = flat / G, head = rec.head * G + flat - token * G;
+    if (token >= s.qn) return;
+    float top = -INFINITY;
+#pragma unroll 4
+    for (int p = 0; p < rec.count; ++p) top = fmaxf(top, part(p)[kRows * DP + 2 * row]);
+    const float safe = top == -INFINITY ? 0.f : top;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
+#pragma unroll 4
+    for (int p = 0; p < rec.count; ++p) {
+      const float2 ml = *reinterpret_cast<const float2*>(part(p) + kRows * DP + 2 * row);
+      const float4 v = *reinterpret_cast<const float4*>(part(p) + row * DP + d);
+      const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2_approx(ml.x - safe);
+      sum = __fmaf_rn(f, ml.y, sum);
+      x.x = __fmaf_rn(f, v.x, x.x);
+      x.y = __fmaf_rn(f, v.y, x.y);
+      x.z = __fmaf_rn(f, v.z, x.z);
+      x.w = __fmaf_rn(f, v.w, x.w);
+    }
+    const float f = sum == 0.f ? 0.f : 1.f / sum;
+    if (d < a.head_size)
+      *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (int64_t)(s.q0 + token) * a.o_token + (int64_t)head * a.o_head + d) =
+          make_uint2(pack2<T>(x.x * f, x.y * f), pack2<T>(x.z * f, x.w * f));
+    if (a.lse && d == 0) a.lse[(int64_t)(s.q0 + token) * a.q_heads + head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+  }
+}
+
+template <typename T, int MODE, int DP> int launch_one(const AttnArgs& a, void* ws, cudaStream_t st) {
+  using C = Cfg<T, MODE, DP>;
+  const char* what = "paged_attention_chunk";
+  auto kernel = chunk_kernel<T, MODE, DP>;
+  if (cudaError_t e = ensure_dynamic_smem((const void*)kernel, C::SMEM); e != cudaSuccess) return set_error(MCOP_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+  const int grid = sm_count(), G = a.q_heads / a.c.kv_heads;
+  Layout w;
+  layout((char*)ws, a.tokens, a.batch, G, DP, grid, &w);
+  launch_pdl(chunk_plan_kernel, dim3(1), dim3(1024), 0, st, a, w, max_tiles(a.tokens, a.batch, G));
+  if (int rc = check_launch(what)) return rc;
+  launch_pdl(kernel, dim3(grid), dim3(kThreads), C::SMEM, st, a, w);
+  if (int rc = check_launch(what)) return rc;
+  launch_pdl(chunk_join_kernel<T, DP>, dim3(grid, kRows / 32), dim3(256), 0, st, a, w);
+  return check_launch(what);
+}
+
+template <typename T, int MODE> int launch_mode(const AttnArgs& a, void* ws, cudaStream_t st) {
+  return a.head_size <= 64 ? launch_one<T, MODE, 64>(a, ws, st) : launch_one<T, MODE, 128>(a, ws, st);
+}
+template <typename T> int launch_type(const AttnArgs& a, void* ws, cudaStream_t st) {
+  if (a.scale_mode == kScaleNone) return launch_mode<T, kScaleNone>(a, ws, st);
+  return a.scale_mode == kScaleHead ? launch_mode<T, kScaleHead>(a, ws, st) : launch_mode<T, kScaleToken>(a, ws, st);
+}
+
+}  // namespace
+
+size_t chunk_workspace(int64_t tokens, int batch, int q_heads, int kv_heads, int head_size) {
+  return layout(nullptr, tokens, batch, q_heads / kv_heads, head_size <= 64 ? 64 : 128, sm_count(), nullptr);
+}
+
+int launch_chunk(const AttnArgs& a, int dtype, void* ws, size_t ws_bytes, cudaStream_t st) {
+  const char* what = "paged_attention_chunk";
+  MCOP_REQUIRE(ws && aligned16(ws) && ws_bytes >= chunk_workspace(a.tokens, a.batch, a.q_heads, a.c.kv_heads, a.head_size), MCOP_ERR_WORKSPACE,
+               "%s: workspace missing, misaligned or too small", what);
+  const double span = (double)a.tokens * a.q_token + (double)a.q_heads * a.q_head;
+  MCOP_REQUIRE((int64_t)a.tokens * a.q_heads <= INT32_MAX && a.q_token >= 0 && a.q_head >= 0 && span < 0x1p34, MCOP_ERR_UNSUPPORTED,
+               "%s: more than 2^31 query rows, or a query that spans more than 2^34 elements", what);
+  return dtype == MCOP_BF16 ? launch_type<__nv_bfloat16>(a, ws, st) : launch_type<__half>(a, ws, st);
+}
+
+}  // namespace mcop
