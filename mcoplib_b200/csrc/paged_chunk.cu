@@ -203,6 +203,15 @@ __device__ __forceinline__ void sts_u4(uint32_t dst, uint32_t x, uint32_t y, uin
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
+// Whether the phase is complete, without waiting for it (try_wait may suspend the thread for microseconds).
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(ok)
+               : "r"(smem_addr(bar)), "r"(parity)
+               : "memory");
+  return ok != 0;
+}
 __device__ __forceinline__ void async_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   if constexpr (ElemTraits<T>::code == MCOP_BF16) {
@@ -275,9 +284,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
   __shared__ int poison[8];               // items whose masked tiles hold a NaN or an infinity in V
   pdl_launch_dependents();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, group = warp >> 2;
-  unsigned char* const smem = raw + (1024 - (smem_addr(raw) & 1023)) % 1024;
-  unsigned char* const q_smem = smem;
-  unsigned char* const ring = smem + 2 * C::TILE;
+  const uint32_t smem = (smem_addr(raw) + 1023) & ~1023u;  // Q: two tiles; then the ring of K and V
   if (tid == 0) {
     for (int i = 0; i < ST; ++i) {
       mbar_init(&bars.full[i], 4);
@@ -360,6 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
 #pragma unroll
         for (int i = 0; i < 128; i += 4) {
           if constexpr (MODE == kScaleToken) {
+            if (i % 32 == 0) asm volatile("" ::: "memory");  // (not all 128 factors in registers at once)
             const float4 f = *reinterpret_cast<const float4*>(&in.ks[i]);
             const float2 p = __fmul2_rn(make_float2(s[i], s[i + 1]), make_float2(f.x, f.y)), q = __fmul2_rn(make_float2(s[i + 2], s[i + 3]), make_float2(f.z, f.w));
             s[i] = p.x; s[i + 1] = p.y; s[i + 2] = q.x; s[i + 3] = q.y;
@@ -393,15 +401,16 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
           }
           if (k > x.k0) {
             // (S of this tile was issued behind the previous tile's P V: that product is complete)
-#pragma unroll
-            for (int i = 0; i < DP / 32; ++i) {
-              float o[32];
-              tmem_ld32(o_addr + 32 * i, o);
+// (8 columns at a time: the logits stay in registers meanwhile)
+#pragma unroll 1
+            for (int i = 0; i < DP; i += 8) {
+              float o[8];
+              tmem_ld8(o_addr + i, o);
               tmem_wait_ld();
-              tmem_loaded32(o);
+              tmem_loaded8(o);
 #pragma unroll
-              for (int d = 0; d < 32; ++d) o[d] *= keep;
-              tmem_st32(o_addr + 32 * i, o);
+              for (int d = 0; d < 8; ++d) o[d] *= keep;
+              tmem_st8(o_addr + i, o);
             }
           }
         }
@@ -514,6 +523,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
     // ------------------------------------------------------------------------------------------ Q, K and V into shared memory
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     const int lt = tid & 127, lwarp = warp & 3;
+    uint32_t q_smem = smem;
+    asm volatile("" : "+r"(q_smem));  // (keeps what the roles derive from it out of the code in front of them)
+    const uint32_t ring = q_smem + 2 * C::TILE;
     const int row_pieces = a.head_size * (C::I8 ? 1 : 2) / 16;  // 16-byte pieces of a cached row
     const uint32_t block16 = (uint32_t)(a.c.block_stride * (C::I8 ? 1 : 2) / 16), page16 = (uint32_t)(a.c.page_stride * (C::I8 ? 1 : 2) / 16),
                    head16 = (uint32_t)(a.c.head_stride * (C::I8 ? 1 : 2) / 16);
@@ -545,9 +557,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
           const int c = lt % C::PIECES;
           bool bad = false;
           for (int row = lt / C::PIECES; row < kTile; row += 128 / C::PIECES) {
-            uint4* p = reinterpret_cast<uint4*>(ring + done.s * C::TILE + (c / 8) * C::HALF + row * 128 + ((c % 8) ^ (row % 8)) * 16);
-            uint4 u = *p;
-            if (not_finite<T>(u)) { *p = u; bad = true; }
+            const uint32_t p = ring + done.s * C::TILE + (c / 8) * C::HALF + row * 128 + ((c % 8) ^ (row % 8)) * 16;
+            uint4 u;
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(p) : "memory");
+            if (not_finite<T>(u)) { sts_u4(p, u.x, u.y, u.z, u.w); bad = true; }
           }
           if (bad) *(volatile int*)&poison[scan_item >> (4 * (pending - 1)) & 7] = 1;
         }
@@ -578,7 +591,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
 
     // Waits for a barrier; copies that have arrived meanwhile are handed over first, since what frees the barrier may need them.
     auto acquire = [&](uint64_t* bar, uint32_t phase) {
-      while (pending > 0 && !__any_sync(0xffffffffu, mbar_try_wait(bar, phase))) {
+      while (pending > 0 && !__any_sync(0xffffffffu, mbar_test(bar, phase))) {
         switch (pending) {
           case 1: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
           case 2: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
@@ -610,7 +623,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
         for (int row = lt / C::PIECES; row < (pt.rows + 127) / 128 * 128; row += 128 / C::PIECES) {
           const uint32_t at = q_at[row];
           const bool live = at != 0xffffffffu && c * 8 < a.head_size;
-          cp_async16(smem_addr(q_smem + (row / 128) * C::TILE + (c / 8) * C::HALF + (row % 128) * 128 + ((c % 8) ^ (row % 8)) * 16),
+          cp_async16(q_smem + (row / 128) * C::TILE + (c / 8) * C::HALF + (row % 128) * 128 + ((c % 8) ^ (row % 8)) * 16,
                      live ? static_cast<const T*>(a.q) + (int64_t)at * 8 + c * 8 : static_cast<const T*>(a.q), live);
         }
       }
@@ -671,14 +684,14 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
           const char* src = kv ? vbase : kbase;
           if constexpr (!C::I8) {
             if (!(ok = acquire(&bars.empty[st.s], st.phase ^ 1))) break;
-            unsigned char* dst = ring + st.s * C::TILE;
+            const uint32_t dst = ring + st.s * C::TILE;
             const int c = lt % C::PIECES;
 #pragma unroll
             for (int i = 0; i < kTile * C::PIECES / 128; ++i) {
               const int row = lt / C::PIECES + i * (128 / C::PIECES);
               const uint32_t at = row_at[buf][row];
               const bool live = at != 0xffffffffu && c < row_pieces;
-              cp_async16(smem_addr(dst + (c / 8) * C::HALF + row * 128 + ((c % 8) ^ (row % 8)) * 16), live ? src + (uint64_t)at * 16 + c * 16 : src, live);
+              cp_async16(dst + (c / 8) * C::HALF + row * 128 + ((c % 8) ^ (row % 8)) * 16, live ? src + (uint64_t)at * 16 + c * 16 : src, live);
             }
             st.advance(ST);
             committed(kv == 0 && k == x.k0, kv == 1 && scan);
@@ -693,7 +706,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
               if (at != 0xffffffffu && c < row_pieces) u[i] = ld_nc_u4(src + (uint64_t)at * 16 + c * 16);
             }
             if (!(ok = mbar_wait_bounded(&bars.empty[st.s], st.phase ^ 1, a.err, kWaitLoad, kSpin))) break;
-            unsigned char* dst = ring + st.s * C::TILE;
+            const uint32_t dst = ring + st.s * C::TILE;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
               const int row = lt / IP + i * (128 / IP);
@@ -708,7 +721,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
                 const int piece = 2 * c + h;
-                sts_u4(smem_addr(dst + (piece / 8) * C::HALF + row * 128 + ((piece % 8) ^ (row % 8)) * 16), y[4 * h], y[4 * h + 1], y[4 * h + 2], y[4 * h + 3]);
+                sts_u4(dst + (piece / 8) * C::HALF + row * 128 + ((piece % 8) ^ (row % 8)) * 16, y[4 * h], y[4 * h + 1], y[4 * h + 2], y[4 * h + 3]);
               }
             }
             if (kv == 0 && k == x.k0) asm volatile("cp.async.wait_all;" ::: "memory");
@@ -733,9 +746,11 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
     // ------------------------------------------------------------------------------------------ the MMAs
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 12 && lane == 0) {
+      uint32_t q_smem = smem;
+      asm volatile("" : "+r"(q_smem));
+      const uint32_t ring = q_smem + 2 * C::TILE;
       constexpr uint32_t QK = f16_idesc(ElemTraits<T>::code == MCOP_BF16, 128, kTile, false);
       constexpr uint32_t PV = f16_idesc(ElemTraits<VT>::code == MCOP_BF16, 128, DP, true);
-      const uint32_t q_addr = smem_addr(q_smem), ring_addr = smem_addr(ring);
       Ring st;
       uint32_t q_phase = 0, p_phase[2] = {0, 0}, oe_phase[2] = {1, 1};
       bool ok = true;
@@ -744,18 +759,18 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
         tc_fence_after();
         return ok;
       };
+      const uint32_t q_low = desc_low(q_smem, 16), k_low = desc_low(ring, 16), v_low = desc_low(ring, C::HALF);
       auto logits = [&](int tile, int stage) {
-#pragma unroll
-        for (int i = 0; i < DP / 16; ++i) {
-          const uint32_t at = (i / 4) * C::HALF + (i % 4) * 32;
-          tc_mma_ss(tmem + tile * 128, smem_desc(q_addr + tile * C::TILE + at, 16, 1024), smem_desc(ring_addr + stage * C::TILE + at, 16, 1024), QK, i > 0);
-        }
+        const uint32_t q = q_low + tile * (C::TILE / 16), k = k_low + stage * (C::TILE / 16);
+        static_for<DP / 16>([&](auto i) {
+          constexpr uint32_t at = (i.value / 4) * C::HALF + (i.value % 4) * 32;
+          tc_mma_ss<QK, at, at>(tmem + tile * 128, q, k, i.value > 0);
+        });
         tc_commit(&bars.s_full[tile]);
       };
       auto values = [&](int tile, int stage, bool more) {
-#pragma unroll
-        for (int i = 0; i < kTile / 16; ++i)
-          tc_mma_ts(tmem + 256 + tile * DP, tmem + tile * 128 + 8 * i, smem_desc(ring_addr + stage * C::TILE + i * 2048, C::HALF, 1024), PV, more || i > 0);
+        const uint32_t v = v_low + stage * (C::TILE / 16);
+        static_for<kTile / 16>([&](auto i) { tc_mma_ts<PV, 8 * i.value, 2048 * i.value>(tmem + 256 + tile * DP, tmem + tile * 128, v, more || i.value > 0); });
       };
       while (ok && line.next(w, a.c.kv_heads, x)) {
         const int two = w.tile[x.tile].rows > 128 ? 2 : 1;

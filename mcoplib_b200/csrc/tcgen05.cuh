@@ -3,6 +3,8 @@
 
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace mcop {
 
 // Allocates / frees all 512 columns of the SM's tensor memory (whole warp); the address goes to shared memory.
@@ -24,12 +26,14 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, float* v) {
                  "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
                : "r"(addr));
 }
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const float* v) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
-               "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr), "f"(v[0]), "f"(v[1]), "f"(v[2]),
-                 "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]), "f"(v[10]), "f"(v[11]), "f"(v[12]),
-                 "f"(v[13]), "f"(v[14]), "f"(v[15]), "f"(v[16]), "f"(v[17]), "f"(v[18]), "f"(v[19]), "f"(v[20]), "f"(v[21]), "f"(v[22]),
-                 "f"(v[23]), "f"(v[24]), "f"(v[25]), "f"(v[26]), "f"(v[27]), "f"(v[28]), "f"(v[29]), "f"(v[30]), "f"(v[31]) : "memory");
+// The same for 8 columns.
+__device__ __forceinline__ void tmem_ld8(uint32_t addr, float* v) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+               : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const float* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]) : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* v) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
@@ -45,6 +49,9 @@ __device__ __forceinline__ void tmem_loaded32(float* v) {
                  "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]),
                  "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31]));
 }
+__device__ __forceinline__ void tmem_loaded8(float* v) {
+  asm volatile("" : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]));
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // Order of tensor-memory accesses across a barrier: before an arrive, after a wait.
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -55,29 +62,40 @@ __device__ __forceinline__ void tc_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"((uint32_t)__cvta_generic_to_shared(bar)) : "memory");
 }
 
-// Descriptor of a shared-memory operand in the 128-byte swizzle: rows of 128 bytes, 8 rows to an atom of 1024 bytes.
-// lbo: bytes between 64-element blocks of the M / N dimension (operands that are contiguous along M / N only);
-// sbo: bytes between atoms.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-  return (uint64_t)((addr & 0x3ffff) >> 4) | (uint64_t)(lbo >> 4) << 16 | (uint64_t)(sbo >> 4) << 32 | 1ull << 46 | 2ull << 61;
-}
+// Descriptor of a shared-memory operand in the 128-byte swizzle: rows of 128 bytes, 8 rows to an atom of 1024 bytes, atoms one behind
+// the other.  The low word: address, and lbo, the bytes between 64-element blocks of the M / N dimension (operands that are
+// contiguous along M / N only).  The high word is the same for all.  Offsets add to the low word in units of 16 bytes.
+__device__ __forceinline__ uint32_t desc_low(uint32_t addr, uint32_t lbo) { return (addr & 0x3ffff) >> 4 | (lbo >> 4) << 16; }
+constexpr uint32_t kDescHigh = 1024 / 16 | 1u << 14 | 2u << 29;
 // Instruction descriptor of kind::f16 with an fp32 accumulator.  bf16: both operands bf16 (otherwise both f16).
 __host__ __device__ constexpr uint32_t f16_idesc(bool bf16, int m, int n, bool b_mn_major) {
   return 1u << 4 | (bf16 ? 1u : 0u) << 7 | (bf16 ? 1u : 0u) << 10 | (b_mn_major ? 1u : 0u) << 16 | (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24;
 }
-// D[tmem] (+)= A[smem] B[smem]
-__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+// D[tmem] (+)= A[smem] B[smem], both operands OFF bytes behind their bases (the additions stay inside: hoisted out of a loop, the
+// descriptors of its products would fill the issuing thread's registers)
+template <uint32_t IDESC, uint32_t A_OFF, uint32_t B_OFF> __device__ __forceinline__ void tc_mma_ss(uint32_t d, uint32_t a, uint32_t b, bool accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+      "{\n\t.reg .pred p;\n\t.reg .b32 x, y, i;\n\t.reg .b64 da, db;\n\tsetp.ne.u32 p, %3, 0;\n\tadd.u32 x, %1, %4;\n\tadd.u32 y, %2, %5;\n\t"
+      "mov.b32 i, %6;\n\tmov.b64 da, {x, %7};\n\tmov.b64 db, {y, %7};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, i, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"((uint32_t)accumulate), "n"(A_OFF / 16), "n"(B_OFF / 16),
+      "n"(IDESC), "r"(kDescHigh)
       : "memory");
 }
-// D[tmem] (+)= A[tmem] B[smem]
-__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+// D[tmem] (+)= A[tmem] B[smem]; A_OFF in columns
+template <uint32_t IDESC, uint32_t A_OFF, uint32_t B_OFF> __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint32_t b, bool accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+      "{\n\t.reg .pred p;\n\t.reg .b32 x, y, i;\n\t.reg .b64 db;\n\tsetp.ne.u32 p, %3, 0;\n\tadd.u32 x, %1, %4;\n\tadd.u32 y, %2, %5;\n\t"
+      "mov.b32 i, %6;\n\tmov.b64 db, {y, %7};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [x], db, i, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"((uint32_t)accumulate), "n"(A_OFF), "n"(B_OFF / 16),
+      "n"(IDESC), "r"(kDescHigh)
       : "memory");
+}
+// Runs f(integral_constant<int, 0>), ..., f(integral_constant<int, N - 1>).
+template <int N, int I = 0, typename F> __device__ __forceinline__ void static_for(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    static_for<N, I + 1>(f);
+  }
 }
 
 }  // namespace mcop
