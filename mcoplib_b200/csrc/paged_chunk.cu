@@ -26,22 +26,29 @@ namespace {
 constexpr int kRows = 256, kTile = 128, kThreads = 512;
 // Fewer tiles than this per CTA are not worth a partial result of their own.
 constexpr int kMinTiles = 2;
-constexpr uint32_t kSpin = 1u << 20;  // tries of a wait
+constexpr uint32_t kSpin = 1u << 20, kPolls = 1u << 26;  // tries of a wait, of a poll that does not suspend the thread
 constexpr int kWaitSoftmax = 8, kWaitLoad = 9, kWaitMma = 10;  // codes of the error word
 
-// The line of work, in the workspace: prefix[i] = 128-token tiles (of one KV head) in front of query tile i.
-struct PlanTile {
-  int b, t, rows, pad;  // sequence, tile of it, rows of the tile that are there
+// The line of work, in the workspace.  A query tile: 256 rows of one sequence, and the tokens that they see between them.
+struct alignas(16) PlanTile {
+  int b, t, rows, q0;      // sequence, tile of it, rows of the tile that are there, first new token of the sequence
+  int qn, len, first, n;   // new tokens, cached tokens; tiles [first, first + n) of 128 tokens reach from lo to hi
+  int lo, hi, pad[2];
+};
+// Where a CTA begins: `left` tiles of 128 tokens from tile k of query tile `tile` and KV head `head` on.
+struct alignas(16) Start {
+  int left, tile, head, k;
 };
 struct Plan {
-  int tiles, pad[3];
+  int64_t share, pad;  // tiles of 128 tokens per CTA
 };
 struct Rec {
   int b, t, head, count;
 };
 struct Layout {  // of the workspace
   Plan* plan;
-  int64_t* prefix;      // [max_tiles + 1]
+  Start* starts;        // [ctas]
+  int64_t* prefix;      // [max_tiles + 1]: tiles of 128 tokens (of one KV head) in front of a query tile
   PlanTile* tile;       // [max_tiles]
   int64_t* seq_tiles;   // [batch + 1]
   Rec* recs;            // [ctas]
@@ -55,6 +62,7 @@ __host__ inline size_t layout(char* ws, int64_t tokens, int batch, int group, in
   auto take = [&](size_t bytes) { const size_t was = at; at += up16(bytes); return ws + was; };
   Layout x;
   x.plan = (Plan*)take(sizeof(Plan));
+  x.starts = (Start*)take(ctas * sizeof(Start));
   x.prefix = (int64_t*)take((mt + 1) * 8);
   x.tile = (PlanTile*)take(mt * sizeof(PlanTile));
   x.seq_tiles = (int64_t*)take((batch + 1) * 8);
@@ -80,7 +88,7 @@ __device__ __forceinline__ Reach reach(const AttnArgs& a, const Seq& s, int t, i
   return r;
 }
 
-__global__ void __launch_bounds__(1024) chunk_plan_kernel(AttnArgs a, Layout w, int64_t limit) {
+__global__ void __launch_bounds__(1024) chunk_plan_kernel(AttnArgs a, Layout w, int64_t limit, int ctas) {
   pdl_launch_dependents();
   pdl_wait();
   __shared__ int64_t sums[33];
@@ -122,7 +130,6 @@ __global__ void __launch_bounds__(1024) chunk_plan_kernel(AttnArgs a, Layout w, 
   const int64_t tiles = min(base, limit);
   if (tid == 0) {
     w.seq_tiles[a.batch] = base;
-    w.plan->tiles = (int)tiles;
   }
   __syncthreads();
   int64_t front = 0;
@@ -138,14 +145,36 @@ __global__ void __launch_bounds__(1024) chunk_plan_kernel(AttnArgs a, Layout w, 
       }
       const int t = (int)(i - w.seq_tiles[lo]);
       const Seq s = sequence<false>(a, lo);
-      w.tile[i] = PlanTile{lo, t, (int)min((int64_t)kRows, (int64_t)s.qn * G - (int64_t)t * kRows), 0};
-      n = reach(a, s, t, G).n;
+      const Reach r = reach(a, s, t, G);
+      n = r.n;
+      w.tile[i] = PlanTile{lo, t, (int)min((int64_t)kRows, (int64_t)s.qn * G - (int64_t)t * kRows), s.q0, s.qn, s.len, r.first, r.n, r.lo, r.hi, {0, 0}};
     }
     const longlong2 s = scan(n);
     if (i < tiles) w.prefix[i] = front + s.x - n;
     front += s.y;
   }
   if (tid == 0) w.prefix[tiles] = front;
+  __syncthreads();
+  // equal shares of the line
+  const int64_t heads = a.c.kv_heads, total = front * heads, share = max((int64_t)kMinTiles, (total + ctas - 1) / ctas);
+  if (tid == 0) w.plan->share = share;
+  for (int c = tid; c < ctas; c += 1024) {
+    const int64_t u = share * c;
+    Start s{(int)max((int64_t)0, min(total - u, share)), 0, 0, 0};
+    if (s.left > 0) {
+      int lo = 0, hi = (int)tiles;  // prefix[lo] * heads <= u < prefix[hi] * heads
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (w.prefix[mid] * heads <= u) lo = mid;
+        else hi = mid;
+      }
+      const int64_t off = u - w.prefix[lo] * heads, n = w.prefix[lo + 1] - w.prefix[lo];
+      s.tile = lo;
+      s.head = (int)(off / n);
+      s.k = (int)(off - s.head * n);
+    }
+    w.starts[c] = s;
+  }
 }
 
 template <typename T, int MODE, int DP> struct Cfg {
@@ -157,39 +186,19 @@ template <typename T, int MODE, int DP> struct Cfg {
   static constexpr int PIECES = DP / 8;                  // 16-byte pieces of a row in shared memory
 };
 
-// A piece of work of a CTA: query tile `tile` of the plan against tiles [k0, k1) of the n of its reach, for one KV head.
-struct Work {
-  int tile, head, k0, k1, n;
-};
+// A piece of work of a CTA: a query tile of the plan against tiles [k0, k1) of the n of its reach, for one KV head.
 struct WorkLine {
-  int left, tile, head, k;  // tiles of 128 tokens still to do; where the next piece begins
-  __device__ __forceinline__ static int64_t total(const Layout& w, int kv_heads) { return w.plan->tiles ? w.prefix[w.plan->tiles] * kv_heads : 0; }
-  __device__ __forceinline__ static int64_t per(int64_t total) { return max((int64_t)kMinTiles, (total + gridDim.x - 1) / gridDim.x); }
-  __device__ __forceinline__ void start(const Layout& w, int kv_heads) {
-    const int64_t all = total(w, kv_heads), share = per(all), u = share * blockIdx.x;
-    left = (int)max((int64_t)0, min(all - u, share));
-    if (left == 0) return;
-    int lo = 0, hi = w.plan->tiles;  // prefix[lo] * kv_heads <= u < prefix[hi] * kv_heads
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (w.prefix[mid] * kv_heads <= u) lo = mid;
-      else hi = mid;
-    }
-    tile = lo;
-    const int64_t off = u - w.prefix[lo] * kv_heads, n = w.prefix[lo + 1] - w.prefix[lo];
-    head = (int)(off / n);
-    k = (int)(off - head * n);
-  }
-  __device__ __forceinline__ bool next(const Layout& w, int kv_heads, Work& x) {
-    if (left <= 0) return false;
-    x.tile = tile;
-    x.head = head;
-    x.n = (int)(w.prefix[tile + 1] - w.prefix[tile]);
-    x.k0 = k;
-    x.k1 = min(x.n, k + left);
-    left -= x.k1 - x.k0;
-    k = 0;
-    if (++head == kv_heads) { head = 0; ++tile; }
+  Start at;
+  int head, k0, k1;
+  __device__ __forceinline__ bool next(const Layout& w, int kv_heads, PlanTile& pt) {
+    if (at.left <= 0) return false;
+    pt = w.tile[at.tile];
+    head = at.head;
+    k0 = at.k;
+    k1 = min(pt.n, at.k + at.left);
+    at.left -= k1 - k0;
+    at.k = 0;
+    if (++at.head == kv_heads) { at.head = 0; ++at.tile; }
     return true;
   }
 };
@@ -309,9 +318,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
   pdl_wait();
   const uint32_t tmem = tmem_at;
   const int G = a.q_heads / a.c.kv_heads;
-  WorkLine line;
-  Work x;
-  line.start(w, a.c.kv_heads);
+  WorkLine x;
+  PlanTile pt;
+  x.at = w.starts[blockIdx.x];
   if (tid == 0) w.recs[blockIdx.x].count = 0;
 
   if (group < 2) {
@@ -324,21 +333,17 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
     uint32_t s_phase = 0, o_phase = 0;
     int item = 0;
     bool ok = true;
-    while (ok && line.next(w, a.c.kv_heads, x)) {
-      const PlanTile pt = w.tile[x.tile];
+    while (ok && x.next(w, a.c.kv_heads, pt)) {
       const bool idle = group == 1 && pt.rows <= 128;
       const int row = group * 128 + r;
       const bool mine = row < pt.rows;
       const int flat = pt.t * kRows + row, token = flat / G, head = x.head * G + flat - token * G;
-      int lo = 0, hi = INT_MAX, first, q0;
-      {
-        const Seq s = sequence<false>(a, pt.b);
-        first = reach(a, s, pt.t, G).first;
-        q0 = s.q0;
-        if (mine) span(a, s, token, lo, hi);
-      }
+      int lo = 0, hi = INT_MAX;
+      if (mine) span(a, Seq{pt.q0, pt.qn, pt.len}, token, lo, hi);
       float c = a.scale * kLog2e;
       if (MODE == kScaleHead) c *= a.c.k_scale[x.head];
+      const bool flip = c < 0.f;  // a negative scale: the largest logit is the smallest product
+      c = c == 0.f ? 1e-37f : fabsf(c);  // (0 times the -inf of a hidden column would be NaN)
       float m = -INFINITY, l = 0.f;
       int e = -1000;
       if (idle) {  // no rows: keep in step with the item
@@ -363,30 +368,39 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
         tmem_wait_ld();
 #pragma unroll
         for (int i = 0; i < 4; ++i) tmem_loaded32(s + 32 * i);
-        // logits in log2 units
+        if constexpr (MODE == kScaleToken) {
+          // logits in log2 units
 #pragma unroll
-        for (int i = 0; i < 128; i += 4) {
-          if constexpr (MODE == kScaleToken) {
+          for (int i = 0; i < 128; i += 4) {
             if (i % 32 == 0) asm volatile("" ::: "memory");  // (not all 128 factors in registers at once)
             const float4 f = *reinterpret_cast<const float4*>(&in.ks[i]);
             const float2 p = __fmul2_rn(make_float2(s[i], s[i + 1]), make_float2(f.x, f.y)), q = __fmul2_rn(make_float2(s[i + 2], s[i + 3]), make_float2(f.z, f.w));
             s[i] = p.x; s[i + 1] = p.y; s[i + 2] = q.x; s[i + 3] = q.y;
-          } else {
-            const float2 p = __fmul2_rn(make_float2(s[i], s[i + 1]), make_float2(c, c)), q = __fmul2_rn(make_float2(s[i + 2], s[i + 3]), make_float2(c, c));
-            s[i] = p.x; s[i + 1] = p.y; s[i + 2] = q.x; s[i + 3] = q.y;
           }
+        } else if (MODE == kScaleHead && flip) {
+#pragma unroll
+          for (int i = 0; i < 128; ++i) s[i] = -s[i];
         }
-        const int base = (first + k) * kTile;
+        const int base = (pt.first + k) * kTile;
         const bool masked = __any_sync(0xffffffffu, base < lo || base + kTile > hi) || !in.all;
         if (masked) {
-          const int from = max(0, min(kTile, lo - base)), to = hi - base;  // columns [from, to) are seen
+          const int from = max(0, lo - base), to = hi - base;  // columns [from, to) are seen
 #pragma unroll
-          for (int i = 0; i < 128; ++i)
-            if (i < from || i >= to || !(in.here[i / 32] >> (i % 32) & 1)) s[i] = -INFINITY;
+          for (int i = 0; i < 4; ++i) {
+            const int f = min(32, max(0, from - 32 * i)), e = min(32, max(0, to - 32 * i));
+            const uint32_t seen = (uint32_t)((1ull << e) - 1) & ~(uint32_t)((1ull << f) - 1) & in.here[i];
+#pragma unroll
+            for (int d = 0; d < 32; ++d) s[32 * i + d] = seen & 1u << d ? s[32 * i + d] : -INFINITY;
+          }
         }
-        float top = fmaxf(s[0], s[1]);
+        float tops[4];
 #pragma unroll
-        for (int i = 2; i < 128; i += 2) asm("max.f32 %0, %0, %1, %2;" : "+f"(top) : "f"(s[i]), "f"(s[i + 1]));
+        for (int j = 0; j < 4; ++j) {
+          tops[j] = fmaxf(s[j], s[j + 4]);
+#pragma unroll
+          for (int i = 8; i < 128; i += 8) asm("max.f32 %0, %0, %1, %2;" : "+f"(tops[j]) : "f"(s[i + j]), "f"(s[i + j + 4]));
+        }
+        const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * (MODE == kScaleToken ? 1.f : c);
         const bool grown = top > m + kMaxSlack;
         const int e_new = in.e;
         const bool moved = MODE == kScaleToken && e_new != e;
@@ -422,8 +436,14 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
 #pragma unroll
           for (int d = 0; d < 16; d += 2) {
             float2 u = make_float2(s[32 * i + 2 * d], s[32 * i + 2 * d + 1]), v = make_float2(s[32 * i + 2 * d + 2], s[32 * i + 2 * d + 3]);
-            u = __fadd2_rn(u, make_float2(-safe, -safe));
-            v = __fadd2_rn(v, make_float2(-safe, -safe));
+            const float2 shift = make_float2(-safe, -safe);
+            if constexpr (MODE == kScaleToken) {
+              u = __fadd2_rn(u, shift);
+              v = __fadd2_rn(v, shift);
+            } else {
+              u = __ffma2_rn(u, make_float2(c, c), shift);
+              v = __ffma2_rn(v, make_float2(c, c), shift);
+            }
             u.x = exp2_approx(u.x); u.y = exp2_approx(u.y);
             v.x = exp2_approx(v.x); v.y = exp2_approx(v.y);
             sum0 = __fadd2_rn(sum0, u);
@@ -454,13 +474,13 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
         if (!(ok = mbar_wait_bounded(&bars.o_full[group], o_phase, a.err, kWaitSoftmax, kSpin))) break;
         o_phase ^= 1;
         tc_fence_after();
-        const bool whole = x.k1 - x.k0 == x.n;
+        const bool whole = x.k1 - x.k0 == pt.n;
         float f = 1.f;
         if (MODE == kScaleToken) f = exp2_approx((float)e);
         if (MODE == kScaleHead) f = a.c.v_scale[x.head];
         const float norm = whole ? (l == 0.f ? 0.f : f / l) : f;
         float* part = w.parts + (int64_t)(2 * blockIdx.x + (x.k0 == 0 ? 1 : 0)) * (kRows * (DP + 2));
-        T* out = static_cast<T*>(a.out) + (int64_t)(q0 + token) * a.o_token + (int64_t)head * a.o_head;
+        T* out = static_cast<T*>(a.out) + (int64_t)(pt.q0 + token) * a.o_token + (int64_t)head * a.o_head;
         const bool sick = !C::I8 && *(volatile int*)&poison[item & 7];
 #pragma unroll 1
         for (int i = 0; i < DP / 32; ++i) {
@@ -477,7 +497,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
           if constexpr (!C::I8) {
             if (sick && mine) {  // the masked tiles were added up without their NaNs and infinities: add those that this row sees
               for (int k = x.k0; k < x.k1; ++k) {
-                const int base = (first + k) * kTile;
+                const int base = (pt.first + k) * kTile;
                 for (int j = max(lo, base); j < min(hi, base + kTile); ++j) {
                   const int slot = slot_of(a, pt.b, j);
                   if (slot < 0) continue;
@@ -510,11 +530,11 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
         }
         if (mine) {
           if (!whole) *reinterpret_cast<float2*>(part + kRows * DP + 2 * row) = make_float2(m, l);
-          else if (a.lse) a.lse[(int64_t)(q0 + token) * a.q_heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+          else if (a.lse) a.lse[(int64_t)(pt.q0 + token) * a.q_heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
         }
       }
-      if (tid == 0 && line.left == 0 && x.k0 == 0 && x.k1 < x.n) {  // the item that begins here and goes on in the next CTA
-        const int64_t share = WorkLine::per(WorkLine::total(w, a.c.kv_heads)), last = share * (blockIdx.x + 1) - 1 + (x.n - x.k1);
+      if (tid == 0 && x.at.left == 0 && x.k0 == 0 && x.k1 < pt.n) {  // the item that begins here and goes on in the next CTA
+        const int64_t share = w.plan->share, last = share * (blockIdx.x + 1) - 1 + (pt.n - x.k1);
         w.recs[blockIdx.x] = Rec{pt.b, pt.t, x.head, (int)(last / share - blockIdx.x) + 1};
       }
       ++item;
@@ -602,12 +622,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
       return mbar_wait_bounded(bar, phase, a.err, kWaitLoad, kSpin);
     };
 
-    while (ok && line.next(w, a.c.kv_heads, x)) {
+    while (ok && x.next(w, a.c.kv_heads, pt)) {
       if (lt == 0) *(volatile int*)&poison[item & 7] = 0;
       // rows of Q
-      const PlanTile pt = w.tile[x.tile];
-      const Seq seq = sequence<false>(a, pt.b);
-      const Reach reached = reach(a, seq, pt.t, G);
+      const Seq seq{pt.q0, pt.qn, pt.len};
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int row = lt + 128 * i, flat = pt.t * kRows + row, token = flat / G;
@@ -637,8 +655,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
       auto look_up = [&](int k) {
         off = -1;
         if (k >= x.k1) return;
-        const int pos = (reached.first + k) * kTile + lt;
-        if (pos < reached.lo || pos >= reached.hi) return;
+        const int pos = (pt.first + k) * kTile + lt;
+        if (pos < pt.lo || pos >= pt.hi) return;
         const int page = a.c.page_of(pos);
         off = pos - page * a.c.block_size;
         block = a.c.tables[pt.b * a.c.table_stride + page];
@@ -677,7 +695,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
         inf.advance(ST);
         look_up(k + 1);
         // --- K, then V
-        const int base = (reached.first + k) * kTile;
+        const int base = (pt.first + k) * kTile;
         const bool scan = base < all_lo || base + kTile > all_hi;
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
@@ -745,17 +763,28 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
   } else {
     // ------------------------------------------------------------------------------------------ the MMAs
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 12 && lane == 0) {
+    if (warp == 12) {
+      // The whole warp walks the loop and one elected thread issues: in uniform code the descriptors live in uniform registers, which
+      // the instruction takes (from a single thread's registers it took 100 cycles to issue a product of 64).
+      constexpr uint32_t kAll = 0xffffffffu;
       uint32_t q_smem = smem;
       asm volatile("" : "+r"(q_smem));
-      const uint32_t ring = q_smem + 2 * C::TILE;
+      q_smem = __reduce_max_sync(kAll, q_smem);
+      const uint32_t at = __reduce_max_sync(kAll, tmem), ring = q_smem + 2 * C::TILE;
       constexpr uint32_t QK = f16_idesc(ElemTraits<T>::code == MCOP_BF16, 128, kTile, false);
       constexpr uint32_t PV = f16_idesc(ElemTraits<VT>::code == MCOP_BF16, 128, DP, true);
       Ring st;
       uint32_t q_phase = 0, p_phase[2] = {0, 0}, oe_phase[2] = {1, 1};
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t phase) {
-        ok = ok && mbar_wait_bounded(bar, phase, a.err, kWaitMma, kSpin);
+        // (polled: a suspended thread wakes late, and everything waits for this one)
+        uint32_t tries = 0;
+        while (ok && !__all_sync(kAll, mbar_test(bar, phase))) {
+          if (++tries == kPolls) {
+            report(a.err, kWaitMma);
+            ok = false;
+          }
+        }
         tc_fence_after();
         return ok;
       };
@@ -763,37 +792,37 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
       auto logits = [&](int tile, int stage) {
         const uint32_t q = q_low + tile * (C::TILE / 16), k = k_low + stage * (C::TILE / 16);
         static_for<DP / 16>([&](auto i) {
-          constexpr uint32_t at = (i.value / 4) * C::HALF + (i.value % 4) * 32;
-          tc_mma_ss<QK, at, at>(tmem + tile * 128, q, k, i.value > 0);
+          constexpr uint32_t off = (i.value / 4) * C::HALF + (i.value % 4) * 32;
+          tc_mma_ss<QK, off, off>(at + tile * 128, q, k, i.value > 0);
         });
         tc_commit(&bars.s_full[tile]);
       };
       auto values = [&](int tile, int stage, bool more) {
         const uint32_t v = v_low + stage * (C::TILE / 16);
-        static_for<kTile / 16>([&](auto i) { tc_mma_ts<PV, 8 * i.value, 2048 * i.value>(tmem + 256 + tile * DP, tmem + tile * 128, v, more || i.value > 0); });
+        static_for<kTile / 16>([&](auto i) { tc_mma_ts<PV, 8 * i.value, 2048 * i.value>(at + 256 + tile * DP, at + tile * 128, v, more || i.value > 0); });
       };
-      while (ok && line.next(w, a.c.kv_heads, x)) {
-        const int two = w.tile[x.tile].rows > 128 ? 2 : 1;
+      while (ok && __any_sync(kAll, x.next(w, a.c.kv_heads, pt))) {
+        const int two = 1 + (int)__reduce_max_sync(kAll, pt.rows > 128), n = __reduce_max_sync(kAll, x.k1 - x.k0);
         if (!wait(&bars.q_full, q_phase)) break;
         q_phase ^= 1;
         if (!wait(&bars.full[st.s], st.phase)) break;
         for (int t = 0; t < two; ++t) logits(t, st.s);
         tc_commit(&bars.empty[st.s]);
-        if (x.k1 - x.k0 == 1) tc_commit(&bars.q_empty);
+        if (n == 1) tc_commit(&bars.q_empty);
         st.advance(ST);
-        for (int k = x.k0; k < x.k1 && ok; ++k) {
+        for (int k = 0; k < n && ok; ++k) {
           Ring v = st;
           st.advance(ST);
-          const bool last = k + 1 == x.k1;
+          const bool last = k + 1 == n;
           if (!wait(&bars.full[v.s], v.phase)) break;
           for (int t = 0; t < two && ok; ++t) {
             if (!wait(&bars.p_full[t], p_phase[t])) break;
             p_phase[t] ^= 1;
-            if (k == x.k0) {  // the item before has left O
+            if (k == 0) {  // the item before has left O
               if (!wait(&bars.o_empty[t], oe_phase[t])) break;
               oe_phase[t] ^= 1;
             }
-            values(t, v.s, k > x.k0);
+            values(t, v.s, k > 0);
             if (last) tc_commit(&bars.o_full[t]);
             else {
               if (t == 0 && !wait(&bars.full[st.s], st.phase)) break;
@@ -809,7 +838,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
           tc_commit(&bars.empty[v.s]);
           if (!last) {
             tc_commit(&bars.empty[st.s]);
-            if (k + 2 == x.k1) tc_commit(&bars.q_empty);
+            if (k + 2 == n) tc_commit(&bars.q_empty);
             st.advance(ST);
           }
         }
@@ -872,7 +901,7 @@ template <typename T, int MODE, int DP> int launch_one(const AttnArgs& a, void* 
   const int grid = sm_count(), G = a.q_heads / a.c.kv_heads;
   Layout w;
   layout((char*)ws, a.tokens, a.batch, G, DP, grid, &w);
-  launch_pdl(chunk_plan_kernel, dim3(1), dim3(1024), 0, st, a, w, max_tiles(a.tokens, a.batch, G));
+  launch_pdl(chunk_plan_kernel, dim3(1), dim3(1024), 0, st, a, w, max_tiles(a.tokens, a.batch, G), grid);
   if (int rc = check_launch(what)) return rc;
   launch_pdl(kernel, dim3(grid), dim3(kThreads), C::SMEM, st, a, w);
   if (int rc = check_launch(what)) return rc;

@@ -57,9 +57,12 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// The mbarrier gets one arrival when every MMA this thread has issued so far is complete.
+// The functions below are called by a whole warp; one elected thread, always the same one, issues.
+// The mbarrier gets one arrival when every MMA issued so far is complete.
 __device__ __forceinline__ void tc_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"((uint32_t)__cvta_generic_to_shared(bar)) : "memory");
+  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
+                   (uint32_t)__cvta_generic_to_shared(bar))
+               : "memory");
 }
 
 // Descriptor of a shared-memory operand in the 128-byte swizzle: rows of 128 bytes, 8 rows to an atom of 1024 bytes, atoms one behind
@@ -75,18 +78,18 @@ __host__ __device__ constexpr uint32_t f16_idesc(bool bf16, int m, int n, bool b
 // descriptors of its products would fill the issuing thread's registers)
 template <uint32_t IDESC, uint32_t A_OFF, uint32_t B_OFF> __device__ __forceinline__ void tc_mma_ss(uint32_t d, uint32_t a, uint32_t b, bool accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b32 x, y, i;\n\t.reg .b64 da, db;\n\tsetp.ne.u32 p, %3, 0;\n\tadd.u32 x, %1, %4;\n\tadd.u32 y, %2, %5;\n\t"
+      "{\n\t.reg .pred p, e;\n\t.reg .b32 x, y, i;\n\t.reg .b64 da, db;\n\tsetp.ne.u32 p, %3, 0;\n\tadd.u32 x, %1, %4;\n\tadd.u32 y, %2, %5;\n\t"
       "mov.b32 i, %6;\n\tmov.b64 da, {x, %7};\n\tmov.b64 db, {y, %7};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, i, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"((uint32_t)accumulate), "n"(A_OFF / 16), "n"(B_OFF / 16),
+      "elect.sync _|e, 0xffffffff;\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, i, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"((uint32_t)accumulate), "n"(A_OFF / 16), "n"(B_OFF / 16),
       "n"(IDESC), "r"(kDescHigh)
       : "memory");
 }
 // D[tmem] (+)= A[tmem] B[smem]; A_OFF in columns
 template <uint32_t IDESC, uint32_t A_OFF, uint32_t B_OFF> __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint32_t b, bool accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b32 x, y, i;\n\t.reg .b64 db;\n\tsetp.ne.u32 p, %3, 0;\n\tadd.u32 x, %1, %4;\n\tadd.u32 y, %2, %5;\n\t"
+      "{\n\t.reg .pred p, e;\n\t.reg .b32 x, y, i;\n\t.reg .b64 db;\n\tsetp.ne.u32 p, %3, 0;\n\tadd.u32 x, %1, %4;\n\tadd.u32 y, %2, %5;\n\t"
       "mov.b32 i, %6;\n\tmov.b64 db, {y, %7};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [x], db, i, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"((uint32_t)accumulate), "n"(A_OFF), "n"(B_OFF / 16),
+      "elect.sync _|e, 0xffffffff;\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], [x], db, i, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"((uint32_t)accumulate), "n"(A_OFF), "n"(B_OFF / 16),
       "n"(IDESC), "r"(kDescHigh)
       : "memory");
 }
