@@ -177,15 +177,6 @@ __global__ void __launch_bounds__(1024) chunk_plan_kernel(AttnArgs a, Layout w, 
   }
 }
 
-template <typename T, int MODE, int DP> struct Cfg {
-  static constexpr bool I8 = MODE != kScaleNone;
-  static constexpr int HALF = kTile * 128;               // 64 columns of 128 rows, 128-byte swizzle
-  static constexpr int TILE = HALF * (DP / 64);          // a 16-bit tile of 128 rows
-  static constexpr int ST = DP == 128 ? 4 : 8;
-  static constexpr int SMEM = 2 * TILE + ST * TILE + 1024;
-  static constexpr int PIECES = DP / 8;                  // 16-byte pieces of a row in shared memory
-};
-
 // A piece of work of a CTA: a query tile of the plan against tiles [k0, k1) of the n of its reach, for one KV head.
 struct WorkLine {
   Start at;
@@ -257,7 +248,7 @@ template <typename T> __device__ __forceinline__ bool not_finite(uint4& u) {
 }
 
 template <int ST> struct Bars {
-  uint64_t full[ST], empty[ST], q_full, q_empty, s_full[2], p_full[2], o_full[2], o_empty[2], info_full[ST], drain;
+  uint64_t full[ST], empty[ST], q_full, q_empty, s_full[2], p_half[2], p_full[2], o_full[2], o_empty[2], info_full[ST], drain;
 };
 struct Ring {
   int s = 0;
@@ -277,23 +268,46 @@ struct TileBits {
   int all, e;
 };
 
+template <typename Info, int ST> struct Control {
+  Info info[ST];
+  Bars<ST> bars;
+  uint32_t row_at[2][kTile];  // cached rows of a tile, in units of 16 bytes
+  uint32_t q_at[kRows];       // rows of a query tile, in units of 8 elements (0xffffffff: none)
+  float vmax[2][4];
+  int poison[8];              // items whose masked tiles hold a NaN or an infinity in V
+  uint32_t tmem_at;
+};
+
+template <typename T, int MODE, int DP> struct Cfg {
+  static constexpr bool I8 = MODE != kScaleNone;
+  static constexpr int HALF = kTile * 128;               // 64 columns of 128 rows, 128-byte swizzle
+  static constexpr int TILE = HALF * (DP / 64);          // a 16-bit tile of 128 rows
+  static constexpr int ST = DP == 128 ? (MODE == kScaleToken ? 4 : 5) : 8;
+  using Info = typename std::conditional<MODE == kScaleToken, TileInfo, TileBits>::type;
+  static constexpr int SMEM = (2 + ST) * TILE + (int)sizeof(Control<Info, ST>);
+  static_assert(SMEM <= 227 * 1024, "shared memory of an SM");
+  static constexpr int PIECES = DP / 8;                  // 16-byte pieces of a row in shared memory
+};
+
 template <typename T, int MODE, int DP>
 __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w) {
   using C = Cfg<T, MODE, DP>;
   using VT = typename std::conditional<C::I8, __half, T>::type;  // type of P and V
-  using Info = typename std::conditional<MODE == kScaleToken, TileInfo, TileBits>::type;
+  using Info = typename C::Info;
   constexpr int ST = C::ST;
-  extern __shared__ __align__(16) unsigned char raw[];
-  __shared__ Bars<ST> bars;
-  __shared__ Info info[ST];
-  __shared__ uint32_t tmem_at;
-  __shared__ uint32_t row_at[2][kTile];   // cached rows of a tile, in units of 16 bytes
-  __shared__ uint32_t q_at[kRows];        // rows of a query tile, in units of 8 elements (0xffffffff: none)
-  __shared__ float vmax[2][4];
-  __shared__ int poison[8];               // items whose masked tiles hold a NaN or an infinity in V
+  using Ctl = Control<Info, ST>;
+  extern __shared__ __align__(1024) unsigned char raw[];  // Q: two tiles; the ring of K and V; control
+  Ctl& ctl = *reinterpret_cast<Ctl*>(raw + (2 + ST) * C::TILE);
+  auto& bars = ctl.bars;
+  auto& info = ctl.info;
+  auto& row_at = ctl.row_at;
+  auto& q_at = ctl.q_at;
+  auto& vmax = ctl.vmax;
+  auto& poison = ctl.poison;
+  uint32_t& tmem_at = ctl.tmem_at;
   pdl_launch_dependents();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, group = warp >> 2;
-  const uint32_t smem = (smem_addr(raw) + 1023) & ~1023u;  // Q: two tiles; then the ring of K and V
+  const uint32_t smem = smem_addr(raw);
   if (tid == 0) {
     for (int i = 0; i < ST; ++i) {
       mbar_init(&bars.full[i], 4);
@@ -304,6 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
     mbar_init(&bars.q_empty, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars.s_full[i], 1);
+      mbar_init(&bars.p_half[i], 4);
       mbar_init(&bars.p_full[i], 4);
       mbar_init(&bars.o_full[i], 1);
       mbar_init(&bars.o_empty[i], 4);
@@ -322,6 +337,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
   PlanTile pt;
   x.at = w.starts[blockIdx.x];
   if (tid == 0) w.recs[blockIdx.x].count = 0;
+  if (smem & 1023) {  // (never seen: the window starts on such a boundary) the swizzle would not match
+    if (tid == 0) report(a.err, kWaitMma);
+    x.at.left = 0;
+  }
 
   if (group < 2) {
     // ------------------------------------------------------------------------------------------ softmax of tile `group`
@@ -462,6 +481,12 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
             p[d + 1] = pack2<VT>(v.x, v.y);
           }
           tmem_st16(s_addr + 16 * i, p);
+          if (i == 1) {  // the product with the first 64 tokens can start
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.p_half[group]);
+          }
         }
         l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
         tmem_wait_st();
@@ -797,9 +822,12 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
         });
         tc_commit(&bars.s_full[tile]);
       };
-      auto values = [&](int tile, int stage, bool more) {
+      auto values = [&](auto half, int tile, int stage, bool more) {
         const uint32_t v = v_low + stage * (C::TILE / 16);
-        static_for<kTile / 16>([&](auto i) { tc_mma_ts<PV, 8 * i.value, 2048 * i.value>(at + 256 + tile * DP, at + tile * 128, v, more || i.value > 0); });
+        static_for<kTile / 32>([&](auto j) {
+          constexpr int i = half.value * (kTile / 32) + j.value;
+          tc_mma_ts<PV, 8 * i, 2048 * i>(at + 256 + tile * DP, at + tile * 128, v, more || i > 0);
+        });
       };
       while (ok && __any_sync(kAll, x.next(w, a.c.kv_heads, pt))) {
         const int two = 1 + (int)__reduce_max_sync(kAll, pt.rows > 128), n = __reduce_max_sync(kAll, x.k1 - x.k0);
@@ -816,13 +844,15 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
           const bool last = k + 1 == n;
           if (!wait(&bars.full[v.s], v.phase)) break;
           for (int t = 0; t < two && ok; ++t) {
-            if (!wait(&bars.p_full[t], p_phase[t])) break;
-            p_phase[t] ^= 1;
+            if (!wait(&bars.p_half[t], p_phase[t])) break;
             if (k == 0) {  // the item before has left O
               if (!wait(&bars.o_empty[t], oe_phase[t])) break;
               oe_phase[t] ^= 1;
             }
-            values(t, v.s, k > 0);
+            values(std::integral_constant<int, 0>{}, t, v.s, k > 0);
+            if (!wait(&bars.p_full[t], p_phase[t])) break;
+            p_phase[t] ^= 1;
+            values(std::integral_constant<int, 1>{}, t, v.s, true);
             if (last) tc_commit(&bars.o_full[t]);
             else {
               if (t == 0 && !wait(&bars.full[st.s], st.phase)) break;
