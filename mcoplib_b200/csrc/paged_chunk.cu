@@ -262,6 +262,7 @@ struct alignas(16) TileInfo {
   float ks[kTile], vs[kTile];  // kScaleToken: K scale times the logit factor, V scale times 2^-e
   uint32_t here[4];            // which tokens are there (their page is in the cache)
   int all, e;                  // all of those inside the reach are; e of the V scales
+  int wild, pad;               // a V scale is not finite
 };
 struct TileBits {
   uint32_t here[4];
@@ -276,6 +277,7 @@ template <typename Info, int ST> struct Control {
   float vmax[2][4];
   int poison[8];              // items whose masked tiles hold a NaN or an infinity in V
   uint32_t tmem_at;
+  alignas(16) float ones[std::is_same<Info, TileInfo>::value ? kTile : 4];
 };
 
 template <typename T, int MODE, int DP> struct Cfg {
@@ -326,6 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
     mbar_init(&bars.drain, 1);
     mbar_init_fence();
   }
+  if (MODE == kScaleToken && tid >= 384) ctl.ones[tid - 384] = 1.f;
   if (warp == 12) tmem_alloc_all(&tmem_at);
   tc_fence_before();
   __syncthreads();
@@ -387,21 +390,17 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
         tmem_wait_ld();
 #pragma unroll
         for (int i = 0; i < 4; ++i) tmem_loaded32(s + 32 * i);
-        if constexpr (MODE == kScaleToken) {
-          // logits in log2 units
-#pragma unroll
-          for (int i = 0; i < 128; i += 4) {
-            if (i % 32 == 0) asm volatile("" ::: "memory");  // (not all 128 factors in registers at once)
-            const float4 f = *reinterpret_cast<const float4*>(&in.ks[i]);
-            const float2 p = __fmul2_rn(make_float2(s[i], s[i + 1]), make_float2(f.x, f.y)), q = __fmul2_rn(make_float2(s[i + 2], s[i + 3]), make_float2(f.z, f.w));
-            s[i] = p.x; s[i + 1] = p.y; s[i + 2] = q.x; s[i + 3] = q.y;
-          }
-        } else if (MODE == kScaleHead && flip) {
+        if (MODE == kScaleHead && flip) {
 #pragma unroll
           for (int i = 0; i < 128; ++i) s[i] = -s[i];
         }
         const int base = (pt.first + k) * kTile;
         const bool masked = __any_sync(0xffffffffu, base < lo || base + kTile > hi) || !in.all;
+        // factors of the columns; where columns are hidden, the products with them are formed here
+        const float* factor = MODE == kScaleToken && masked ? ctl.ones : nullptr;
+        if constexpr (MODE == kScaleToken) {
+          if (!masked) factor = in.ks;
+        }
         if (masked) {
           const int from = max(0, lo - base), to = hi - base;  // columns [from, to) are seen
 #pragma unroll
@@ -409,15 +408,29 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
             const int f = min(32, max(0, from - 32 * i)), e = min(32, max(0, to - 32 * i));
             const uint32_t seen = (uint32_t)((1ull << e) - 1) & ~(uint32_t)((1ull << f) - 1) & in.here[i];
 #pragma unroll
-            for (int d = 0; d < 32; ++d) s[32 * i + d] = seen & 1u << d ? s[32 * i + d] : -INFINITY;
+            for (int d = 0; d < 32; ++d) {
+              float v = s[32 * i + d];
+              if constexpr (MODE == kScaleToken) v *= in.ks[32 * i + d];
+              s[32 * i + d] = seen & 1u << d ? v : -INFINITY;
+            }
           }
         }
-        float tops[4];
+        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          tops[j] = fmaxf(s[j], s[j + 4]);
+        for (int i = 0; i < 128; i += 8) {
+          if constexpr (MODE == kScaleToken) {
+            if (i % 32 == 0) asm volatile("" ::: "memory");  // (not all 128 factors in registers at once)
 #pragma unroll
-          for (int i = 8; i < 128; i += 8) asm("max.f32 %0, %0, %1, %2;" : "+f"(tops[j]) : "f"(s[i + j]), "f"(s[i + j + 4]));
+            for (int j = 0; j < 8; j += 4) {
+              const float4 f = *reinterpret_cast<const float4*>(factor + i + j);
+              const float2 u = __fmul2_rn(make_float2(s[i + j], s[i + j + 1]), make_float2(f.x, f.y)), v = __fmul2_rn(make_float2(s[i + j + 2], s[i + j + 3]), make_float2(f.z, f.w));
+              asm("max.f32 %0, %0, %1, %2;" : "+f"(tops[j / 2]) : "f"(u.x), "f"(u.y));
+              asm("max.f32 %0, %0, %1, %2;" : "+f"(tops[j / 2 + 1]) : "f"(v.x), "f"(v.y));
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) asm("max.f32 %0, %0, %1, %2;" : "+f"(tops[j]) : "f"(s[i + j]), "f"(s[i + j + 4]));
+          }
         }
         const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * (MODE == kScaleToken ? 1.f : c);
         const bool grown = top > m + kMaxSlack;
@@ -457,8 +470,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
             float2 u = make_float2(s[32 * i + 2 * d], s[32 * i + 2 * d + 1]), v = make_float2(s[32 * i + 2 * d + 2], s[32 * i + 2 * d + 3]);
             const float2 shift = make_float2(-safe, -safe);
             if constexpr (MODE == kScaleToken) {
-              u = __fadd2_rn(u, shift);
-              v = __fadd2_rn(v, shift);
+              const float4 f = *reinterpret_cast<const float4*>(factor + 32 * i + 2 * d);
+              u = __ffma2_rn(u, make_float2(f.x, f.y), shift);
+              v = __ffma2_rn(v, make_float2(f.z, f.w), shift);
             } else {
               u = __ffma2_rn(u, make_float2(c, c), shift);
               v = __ffma2_rn(v, make_float2(c, c), shift);
@@ -469,7 +483,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
             sum1 = __fadd2_rn(sum1, v);
             if constexpr (MODE == kScaleToken) {
               const float4 f = *reinterpret_cast<const float4*>(&in.vs[32 * i + 2 * d]);
-              if (masked) {  // a scale that is not finite reaches only the rows that see its token
+              if (in.wild) {  // a scale that is not finite reaches only the rows that see its token
                 u.x = u.x == 0.f ? 0.f : u.x * f.x; u.y = u.y == 0.f ? 0.f : u.y * f.y;
                 v.x = v.x == 0.f ? 0.f : v.x * f.z; v.y = v.y == 0.f ? 0.f : v.y * f.w;
               } else {
@@ -699,11 +713,20 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
           const int64_t at = here ? ((int64_t)block * a.c.block_size + off) * a.c.kv_heads + x.head : 0;
           if (here) { ks = a.c.k_scale[at]; vs = a.c.v_scale[at]; }
           const float top = warp_max(fabsf(vs) <= FLT_MAX ? fabsf(vs) : 0.f);
-          if (lane == 0) vmax[buf][lwarp] = top;
+          const bool wild = __any_sync(0xffffffffu, !(fabsf(vs) <= FLT_MAX));
+          if (lane == 0) vmax[buf][lwarp] = wild ? -1.f - top : top;
         }
         const bool sound = sync_and(off < 0 || known);
         if constexpr (MODE == kScaleToken) {
-          const float top = fmaxf(fmaxf(vmax[buf][0], vmax[buf][1]), fmaxf(vmax[buf][2], vmax[buf][3]));
+          float top = 0.f;
+          bool wild = false;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float v = vmax[buf][i];
+            wild |= v < 0.f;
+            top = fmaxf(top, v < 0.f ? -1.f - v : v);
+          }
+          if (lt == 0) in.wild = wild;
           // 2^e >= the tile's largest scale; moved only upwards and by more than 2^6, so that weight times scale stays below
           // 2^14 (f16 ends at 2^16) and O is rescaled rarely
           const int need = max((int)(__float_as_uint(top) >> 23) - 126, -100);
