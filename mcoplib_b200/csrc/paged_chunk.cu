@@ -222,18 +222,25 @@ template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float 
     return *reinterpret_cast<uint32_t*>(&h);
   }
 }
-// Two codes (bytes 0 and 2 of x) as a pair of T, exactly: 128 + seven bits minus 128 or 256 in bf16, 1024 + (code + 128) in f16.
-template <typename T> __device__ __forceinline__ uint32_t codes2(uint32_t x) {
-  if constexpr (ElemTraits<T>::code == MCOP_BF16) {
-    const uint32_t lo = (x & 0x007f007fu) | 0x43004300u, hi = (x & 0x00800080u) | 0x43004300u;
-    __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&lo), *reinterpret_cast<const __nv_bfloat162*>(&hi));
-    return *reinterpret_cast<uint32_t*>(&r);
-  } else {
-    const uint32_t u = (x & 0x00ff00ffu) ^ 0x64806480u, off = 0x64806480u;
-    __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&u), *reinterpret_cast<const __half2*>(&off));
-    return *reinterpret_cast<uint32_t*>(&r);
+// Two codes (bytes 0 and 2 of x, the others ignored) as a pair of T, exactly: 128 + seven bits minus 128 or 256 in bf16, 1024 +
+// (code + 128) in f16.  The masks stay in registers: as immediates each would cost an instruction of its own.
+struct Codes {
+  uint32_t m7 = 0x007f007fu, m1 = 0x00800080u, one = 0x43004300u, m8 = 0x00ff00ffu, bias = 0x64806480u;
+  __device__ __forceinline__ Codes() { asm volatile("" : "+r"(m7), "+r"(m1), "+r"(one), "+r"(m8), "+r"(bias)); }
+  template <typename T> __device__ __forceinline__ uint32_t two(uint32_t x) const {
+    uint32_t lo, hi;
+    if constexpr (ElemTraits<T>::code == MCOP_BF16) {
+      asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(lo) : "r"(x), "r"(m7), "r"(one));  // (x & mask) | one
+      asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(hi) : "r"(x), "r"(m1), "r"(one));
+      __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&lo), *reinterpret_cast<const __nv_bfloat162*>(&hi));
+      return *reinterpret_cast<uint32_t*>(&r);
+    } else {
+      asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(lo) : "r"(x), "r"(m8), "r"(bias));  // (x & mask) ^ bias
+      __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&lo), *reinterpret_cast<const __half2*>(&bias));
+      return *reinterpret_cast<uint32_t*>(&r);
+    }
   }
-}
+};
 // Whether one of the eight 16-bit floats is a NaN or an infinity; `clean` gets them with those replaced by 0.
 template <typename T> __device__ __forceinline__ bool not_finite(uint4& u) {
   constexpr uint32_t E = ElemTraits<T>::code == MCOP_BF16 ? 0x7f80u : 0x7c00u;
@@ -247,8 +254,8 @@ template <typename T> __device__ __forceinline__ bool not_finite(uint4& u) {
   return bad;
 }
 
-template <int ST> struct Bars {
-  uint64_t full[ST], empty[ST], q_full, q_empty, s_full[2], p_half[2], p_full[2], o_full[2], o_empty[2], info_full[ST], drain;
+template <int ST, int NI> struct Bars {
+  uint64_t full[ST], empty[ST], q_full, q_empty, s_full[2], p_half[2], p_full[2], o_full[2], o_empty[2], info_full[NI], drain;
 };
 struct Ring {
   int s = 0;
@@ -269,9 +276,9 @@ struct TileBits {
   int all, e;
 };
 
-template <typename Info, int ST> struct Control {
-  Info info[ST];
-  Bars<ST> bars;
+template <typename Info, int ST, int NI> struct Control {
+  Info info[NI];
+  Bars<ST, NI> bars;
   uint32_t row_at[2][kTile];  // cached rows of a tile, in units of 16 bytes
   uint32_t q_at[kRows];       // rows of a query tile, in units of 8 elements (0xffffffff: none)
   float vmax[2][4];
@@ -284,9 +291,11 @@ template <typename T, int MODE, int DP> struct Cfg {
   static constexpr bool I8 = MODE != kScaleNone;
   static constexpr int HALF = kTile * 128;               // 64 columns of 128 rows, 128-byte swizzle
   static constexpr int TILE = HALF * (DP / 64);          // a 16-bit tile of 128 rows
-  static constexpr int ST = DP == 128 ? (MODE == kScaleToken ? 4 : 5) : 8;
+  static constexpr int RAW = I8 ? 2 * kTile * DP : 0;     // two int8 tiles on their way
+  static constexpr int ST = DP == 128 ? (MODE == kScaleToken ? 3 : I8 ? 4 : 5) : 8;
+  static constexpr int NI = ST < 4 ? 4 : ST;             // tiles whose information is kept
   using Info = typename std::conditional<MODE == kScaleToken, TileInfo, TileBits>::type;
-  static constexpr int SMEM = (2 + ST) * TILE + (int)sizeof(Control<Info, ST>);
+  static constexpr int SMEM = (2 + ST) * TILE + RAW + (int)sizeof(Control<Info, ST, NI>);
   static_assert(SMEM <= 227 * 1024, "shared memory of an SM");
   static constexpr int PIECES = DP / 8;                  // 16-byte pieces of a row in shared memory
 };
@@ -297,9 +306,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
   using VT = typename std::conditional<C::I8, __half, T>::type;  // type of P and V
   using Info = typename C::Info;
   constexpr int ST = C::ST;
-  using Ctl = Control<Info, ST>;
+  using Ctl = Control<Info, C::ST, C::NI>;
   extern __shared__ __align__(1024) unsigned char raw[];  // Q: two tiles; the ring of K and V; control
-  Ctl& ctl = *reinterpret_cast<Ctl*>(raw + (2 + ST) * C::TILE);
+  Ctl& ctl = *reinterpret_cast<Ctl*>(raw + (2 + ST) * C::TILE + C::RAW);
   auto& bars = ctl.bars;
   auto& info = ctl.info;
   auto& row_at = ctl.row_at;
@@ -314,8 +323,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
     for (int i = 0; i < ST; ++i) {
       mbar_init(&bars.full[i], 4);
       mbar_init(&bars.empty[i], 1);
-      mbar_init(&bars.info_full[i], 4);
     }
+    for (int i = 0; i < C::NI; ++i) mbar_init(&bars.info_full[i], 4);
     mbar_init(&bars.q_full, 4);
     mbar_init(&bars.q_empty, 1);
     for (int i = 0; i < 2; ++i) {
@@ -371,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
       if (idle) {  // no rows: keep in step with the item
         if (!(ok = mbar_wait_bounded(&bars.o_full[group], o_phase, a.err, kWaitSoftmax, kSpin))) break;
         o_phase ^= 1;
-        for (int k = x.k0; k < x.k1; ++k) inf.advance(ST);
+        for (int k = x.k0; k < x.k1; ++k) inf.advance(C::NI);
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.o_empty[group]);
         ++item;
@@ -380,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
       for (int k = x.k0; k < x.k1 && ok; ++k) {
         const Info& in = info[inf.s];
         if (!(ok = mbar_wait_bounded(&bars.info_full[inf.s], inf.phase, a.err, kWaitSoftmax, kSpin))) break;
-        inf.advance(ST);
+        inf.advance(C::NI);
         if (!(ok = mbar_wait_bounded(&bars.s_full[group], s_phase, a.err, kWaitSoftmax, kSpin))) break;
         s_phase ^= 1;
         tc_fence_after();
@@ -601,6 +610,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
       return r != 0;
     };
     Ring st, done, inf;       // stage to fill next, stage to hand over next, tile information to fill next
+    const uint32_t rawbuf = ring + ST * C::TILE;
+    const Codes codes;
     uint32_t q_phase = 0;
     int pending = 0;          // copies issued and not handed over (float caches)
     uint32_t with_q = 0, scan_v = 0;  // one bit per pending copy, the oldest in bit pending - 1: Q came with it; V of a masked tile
@@ -701,8 +712,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
         block = a.c.tables[pt.b * a.c.table_stride + page];
       };
       look_up(x.k0);
-      for (int k = x.k0; k < x.k1 && ok; ++k) {
-        // --- where the tile's rows are, and what the softmax needs to know of them
+      // where the rows of tile k are, and what the softmax needs to know of them
+      auto prepare = [&](int k) {
         const bool known = (uint32_t)block < (uint32_t)a.c.num_blocks, here = off >= 0 && known;
         if (off >= 0 && !known) report(a.err, MCOP_DEVERR_SLOT);
         row_at[buf][lt] = here ? (uint32_t)block * block16 + (uint32_t)off * page16 + (uint32_t)x.head * head16 : 0xffffffffu;
@@ -740,15 +751,17 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.info_full[inf.s]);
-        inf.advance(ST);
+        inf.advance(C::NI);
         look_up(k + 1);
-        // --- K, then V
-        const int base = (pt.first + k) * kTile;
-        const bool scan = base < all_lo || base + kTile > all_hi;
+      };
+      if constexpr (!C::I8) {
+        for (int k = x.k0; k < x.k1 && ok; ++k) {
+          prepare(k);
+          const int base = (pt.first + k) * kTile;
+          const bool scan = base < all_lo || base + kTile > all_hi;
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          const char* src = kv ? vbase : kbase;
-          if constexpr (!C::I8) {
+          for (int kv = 0; kv < 2; ++kv) {
+            const char* src = kv ? vbase : kbase;
             if (!(ok = acquire(&bars.empty[st.s], st.phase ^ 1))) break;
             const uint32_t dst = ring + st.s * C::TILE;
             const int c = lt % C::PIECES;
@@ -761,46 +774,71 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
             }
             st.advance(ST);
             committed(kv == 0 && k == x.k0, kv == 1 && scan);
-          } else {
-            constexpr int IP = DP / 16, N = kTile * IP / 128;  // 16-byte pieces of an int8 row; pieces per thread
-            const int c = lt % IP;
-            uint4 u[N];
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-              const uint32_t at = row_at[buf][lt / IP + i * (128 / IP)];
-              u[i] = make_uint4(0, 0, 0, 0);
-              if (at != 0xffffffffu && c < row_pieces) u[i] = ld_nc_u4(src + (uint64_t)at * 16 + c * 16);
-            }
-            if (!(ok = mbar_wait_bounded(&bars.empty[st.s], st.phase ^ 1, a.err, kWaitLoad, kSpin))) break;
-            const uint32_t dst = ring + st.s * C::TILE;
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-              const int row = lt / IP + i * (128 / IP);
-              const uint32_t wd[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
-              uint32_t y[8];
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const uint32_t p = __byte_perm(wd[j], 0, 0x4140), q = __byte_perm(wd[j], 0, 0x4342);
-                y[2 * j] = kv ? codes2<VT>(p) : codes2<T>(p);
-                y[2 * j + 1] = kv ? codes2<VT>(q) : codes2<T>(q);
-              }
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const int piece = 2 * c + h;
-                sts_u4(dst + (piece / 8) * C::HALF + row * 128 + ((piece % 8) ^ (row % 8)) * 16, y[4 * h], y[4 * h + 1], y[4 * h + 2], y[4 * h + 3]);
-              }
-            }
-            if (kv == 0 && k == x.k0) asm volatile("cp.async.wait_all;" ::: "memory");
-            async_proxy_fence();
-            __syncwarp();
-            if (lane == 0) {
-              if (kv == 0 && k == x.k0) mbar_arrive(&bars.q_full);
-              mbar_arrive(&bars.full[st.s]);
-            }
-            st.advance(ST);
           }
+          buf ^= 1;
         }
-        buf ^= 1;
+      } else {
+        // int8 rows come by asynchronous copy, a tile ahead of the conversion; a thread converts the pieces that it has copied
+        constexpr int IP = DP / 16, N = kTile * IP / 128;  // 16-byte pieces of a row; pieces per thread
+        const int c = lt % IP;
+        auto fetch = [&](int kv) {  // K (0) or V (1) of the tile prepared last
+          const char* src = kv ? vbase : kbase;
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            const uint32_t at = row_at[buf][lt / IP + i * (128 / IP)];
+            const bool live = at != 0xffffffffu && c < row_pieces;
+            cp_async16(rawbuf + kv * (kTile * DP) + (i * 128 + lt) * 16, live ? src + (uint64_t)at * 16 + c * 16 : src, live);
+          }
+          asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        auto convert = [&](auto which, bool with_q) {
+          constexpr int kv = decltype(which)::value;
+          if (!(ok = mbar_wait_bounded(&bars.empty[st.s], st.phase ^ 1, a.err, kWaitLoad, kSpin))) return;
+          const uint32_t dst = ring + st.s * C::TILE, from = rawbuf + kv * (kTile * DP) + lt * 16;
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            const int row = lt / IP + i * (128 / IP);
+            uint32_t wd[4], y[8];
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(wd[0]), "=r"(wd[1]), "=r"(wd[2]), "=r"(wd[3]) : "r"(from + i * 2048) : "memory");
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t p = __byte_perm(wd[j], 0, 0x4140), q = __byte_perm(wd[j], 0, 0x4342);
+              y[2 * j] = kv ? codes.template two<VT>(p) : codes.template two<T>(p);
+              y[2 * j + 1] = kv ? codes.template two<VT>(q) : codes.template two<T>(q);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int piece = 2 * c + h;
+              sts_u4(dst + (piece / 8) * C::HALF + row * 128 + ((piece % 8) ^ (row % 8)) * 16, y[4 * h], y[4 * h + 1], y[4 * h + 2], y[4 * h + 3]);
+            }
+          }
+          async_proxy_fence();
+          __syncwarp();
+          if (lane == 0) {
+            if (with_q) mbar_arrive(&bars.q_full);
+            mbar_arrive(&bars.full[st.s]);
+          }
+          st.advance(ST);
+        };
+        prepare(x.k0);
+        fetch(0);  // (Q is in the same group)
+        fetch(1);
+        for (int k = x.k0; k < x.k1 && ok; ++k) {
+          const bool more = k + 1 < x.k1;
+          asm volatile("cp.async.wait_group 1;" ::: "memory");
+          convert(std::integral_constant<int, 0>{}, k == x.k0);
+          if (!ok) break;
+          buf ^= 1;
+          if (more) {
+            prepare(k + 1);
+            fetch(0);
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+          } else {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+          }
+          convert(std::integral_constant<int, 1>{}, false);
+          if (more && ok) fetch(1);
+        }
       }
       ++item;
     }
