@@ -269,7 +269,8 @@ struct alignas(16) TileInfo {
   float ks[kTile], vs[kTile];  // kScaleToken: K scale times the logit factor, V scale times 2^-e
   uint32_t here[4];            // which tokens are there (their page is in the cache)
   int all, e;                  // all of those inside the reach are; e of the V scales
-  int wild, pad;               // a V scale is not finite
+  int wild, odd;               // a V scale is not finite; a K scale is not, or is negative
+  float kmax, pad[3];          // the largest factor
 };
 struct TileBits {
   uint32_t here[4];
@@ -281,7 +282,7 @@ template <typename Info, int ST, int NI> struct Control {
   Bars<ST, NI> bars;
   uint32_t row_at[2][kTile];  // cached rows of a tile, in units of 16 bytes
   uint32_t q_at[kRows];       // rows of a query tile, in units of 8 elements (0xffffffff: none)
-  float vmax[2][4];
+  float vmax[2][4], kmax[2][4];
   int poison[8];              // items whose masked tiles hold a NaN or an infinity in V
   uint32_t tmem_at;
   alignas(16) float ones[std::is_same<Info, TileInfo>::value ? kTile : 4];
@@ -314,6 +315,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
   auto& row_at = ctl.row_at;
   auto& q_at = ctl.q_at;
   auto& vmax = ctl.vmax;
+  auto& kmax = ctl.kmax;
   auto& poison = ctl.poison;
   uint32_t& tmem_at = ctl.tmem_at;
   pdl_launch_dependents();
@@ -427,21 +429,31 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
         float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int i = 0; i < 128; i += 8) {
-          if constexpr (MODE == kScaleToken) {
-            if (i % 32 == 0) asm volatile("" ::: "memory");  // (not all 128 factors in registers at once)
 #pragma unroll
-            for (int j = 0; j < 8; j += 4) {
-              const float4 f = *reinterpret_cast<const float4*>(factor + i + j);
-              const float2 u = __fmul2_rn(make_float2(s[i + j], s[i + j + 1]), make_float2(f.x, f.y)), v = __fmul2_rn(make_float2(s[i + j + 2], s[i + j + 3]), make_float2(f.z, f.w));
-              asm("max.f32 %0, %0, %1, %2;" : "+f"(tops[j / 2]) : "f"(u.x), "f"(u.y));
-              asm("max.f32 %0, %0, %1, %2;" : "+f"(tops[j / 2 + 1]) : "f"(v.x), "f"(v.y));
-            }
-          } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) asm("max.f32 %0, %0, %1, %2;" : "+f"(tops[j]) : "f"(s[i + j]), "f"(s[i + j + 4]));
-          }
+          for (int j = 0; j < 4; ++j) asm("max.f32 %0, %0, %1, %2;" : "+f"(tops[j]) : "f"(s[i + j]), "f"(s[i + j + 4]));
         }
-        const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * (MODE == kScaleToken ? 1.f : c);
+        float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+        if constexpr (MODE == kScaleToken) {
+          // The largest product, times the largest factor, bounds the logits; they are looked at one by one only where the
+          // bound would move the maximum.
+          if (!masked) {
+            top = fmaxf(top, 0.f) * in.kmax;
+            if (__any_sync(0xffffffffu, top > m + kMaxSlack) || in.odd) {
+              float2 best = make_float2(-INFINITY, -INFINITY);
+#pragma unroll
+              for (int i = 0; i < 128; i += 4) {
+                if (i % 32 == 0) asm volatile("" ::: "memory");  // (not all 128 factors in registers at once)
+                const float4 f = *reinterpret_cast<const float4*>(&in.ks[i]);
+                const float2 u = __fmul2_rn(make_float2(s[i], s[i + 1]), make_float2(f.x, f.y)), v = __fmul2_rn(make_float2(s[i + 2], s[i + 3]), make_float2(f.z, f.w));
+                asm("max.f32 %0, %0, %1, %2;" : "+f"(best.x) : "f"(u.x), "f"(u.y));
+                asm("max.f32 %0, %0, %1, %2;" : "+f"(best.y) : "f"(v.x), "f"(v.y));
+              }
+              top = fmaxf(best.x, best.y);
+            }
+          }
+        } else {
+          top *= c;
+        }
         const bool grown = top > m + kMaxSlack;
         const int e_new = in.e;
         const bool moved = MODE == kScaleToken && e_new != e;
@@ -725,7 +737,12 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
           if (here) { ks = a.c.k_scale[at]; vs = a.c.v_scale[at]; }
           const float top = warp_max(fabsf(vs) <= FLT_MAX ? fabsf(vs) : 0.f);
           const bool wild = __any_sync(0xffffffffu, !(fabsf(vs) <= FLT_MAX));
-          if (lane == 0) vmax[buf][lwarp] = wild ? -1.f - top : top;
+          const bool odd = __any_sync(0xffffffffu, !(ks >= 0.f && ks <= FLT_MAX));
+          const float ktop = warp_max(ks >= 0.f && ks <= FLT_MAX ? ks : 0.f);
+          if (lane == 0) {
+            vmax[buf][lwarp] = wild ? -1.f - top : top;
+            kmax[buf][lwarp] = odd ? -1.f : ktop;
+          }
         }
         const bool sound = sync_and(off < 0 || known);
         if constexpr (MODE == kScaleToken) {
@@ -737,7 +754,12 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
             wild |= v < 0.f;
             top = fmaxf(top, v < 0.f ? -1.f - v : v);
           }
-          if (lt == 0) in.wild = wild;
+          const float ktop = fmaxf(fmaxf(kmax[buf][0], kmax[buf][1]), fmaxf(kmax[buf][2], kmax[buf][3])), klow = fminf(fminf(kmax[buf][0], kmax[buf][1]), fminf(kmax[buf][2], kmax[buf][3]));
+          if (lt == 0) {
+            in.wild = wild;
+            in.odd = klow < 0.f;
+            in.kmax = ktop * (a.scale * kLog2e) * (1.f + 0x1p-20f);
+          }
           // 2^e >= the tile's largest scale; moved only upwards and by more than 2^6, so that weight times scale stays below
           // 2^14 (f16 ends at 2^16) and O is rescaled rarely
           const int need = max((int)(__float_as_uint(top) >> 23) - 126, -100);
