@@ -203,6 +203,11 @@ __device__ __forceinline__ void sts_u4(uint32_t dst, uint32_t x, uint32_t y, uin
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
+__device__ __forceinline__ float4 lds4(uint32_t a) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a));
+  return v;
+}
 // Whether the phase is complete, without waiting for it (try_wait may suspend the thread for microseconds).
 __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
@@ -408,9 +413,12 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
         const int base = (pt.first + k) * kTile;
         const bool masked = __any_sync(0xffffffffu, base < lo || base + kTile > hi) || !in.all;
         // factors of the columns; where columns are hidden, the products with them are formed here
-        const float* factor = MODE == kScaleToken && masked ? ctl.ones : nullptr;
+        uint32_t factor = 0, vfactor = 0;
+        bool wild = false;
         if constexpr (MODE == kScaleToken) {
-          if (!masked) factor = in.ks;
+          factor = smem_addr(masked ? ctl.ones : in.ks);
+          vfactor = smem_addr(in.vs);
+          wild = in.wild;
         }
         if (masked) {
           const int from = max(0, lo - base), to = hi - base;  // columns [from, to) are seen
@@ -443,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
 #pragma unroll
               for (int i = 0; i < 128; i += 4) {
                 if (i % 32 == 0) asm volatile("" ::: "memory");  // (not all 128 factors in registers at once)
-                const float4 f = *reinterpret_cast<const float4*>(&in.ks[i]);
+                const float4 f = lds4(factor + 4 * i);
                 const float2 u = __fmul2_rn(make_float2(s[i], s[i + 1]), make_float2(f.x, f.y)), v = __fmul2_rn(make_float2(s[i + 2], s[i + 3]), make_float2(f.z, f.w));
                 asm("max.f32 %0, %0, %1, %2;" : "+f"(best.x) : "f"(u.x), "f"(u.y));
                 asm("max.f32 %0, %0, %1, %2;" : "+f"(best.y) : "f"(v.x), "f"(v.y));
@@ -483,15 +491,14 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
         }
         const float safe = m == -INFINITY ? 0.f : m;
         float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t p[16];
+        // 32 weights: rounded, summed, times their tokens' scales.  FIX: a scale that is not finite reaches only the rows that see its token.
+        auto weights = [&](auto FIX, int i, uint32_t* p) {
+          const float2 shift = make_float2(-safe, -safe);
 #pragma unroll
           for (int d = 0; d < 16; d += 2) {
             float2 u = make_float2(s[32 * i + 2 * d], s[32 * i + 2 * d + 1]), v = make_float2(s[32 * i + 2 * d + 2], s[32 * i + 2 * d + 3]);
-            const float2 shift = make_float2(-safe, -safe);
             if constexpr (MODE == kScaleToken) {
-              const float4 f = *reinterpret_cast<const float4*>(factor + 32 * i + 2 * d);
+              const float4 f = lds4(factor + 4 * (32 * i + 2 * d));
               u = __ffma2_rn(u, make_float2(f.x, f.y), shift);
               v = __ffma2_rn(v, make_float2(f.z, f.w), shift);
             } else {
@@ -503,18 +510,25 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
             sum0 = __fadd2_rn(sum0, u);
             sum1 = __fadd2_rn(sum1, v);
             if constexpr (MODE == kScaleToken) {
-              const float4 f = *reinterpret_cast<const float4*>(&in.vs[32 * i + 2 * d]);
-              if (in.wild) {  // a scale that is not finite reaches only the rows that see its token
-                u.x = u.x == 0.f ? 0.f : u.x * f.x; u.y = u.y == 0.f ? 0.f : u.y * f.y;
-                v.x = v.x == 0.f ? 0.f : v.x * f.z; v.y = v.y == 0.f ? 0.f : v.y * f.w;
+              const float4 f = lds4(vfactor + 4 * (32 * i + 2 * d));
+              const float2 y = __fmul2_rn(u, make_float2(f.x, f.y)), z = __fmul2_rn(v, make_float2(f.z, f.w));
+              if constexpr (decltype(FIX)::value) {
+                u.x = u.x == 0.f ? 0.f : y.x; u.y = u.y == 0.f ? 0.f : y.y;
+                v.x = v.x == 0.f ? 0.f : z.x; v.y = v.y == 0.f ? 0.f : z.y;
               } else {
-                u = __fmul2_rn(u, make_float2(f.x, f.y));
-                v = __fmul2_rn(v, make_float2(f.z, f.w));
+                u = y;
+                v = z;
               }
             }
             p[d] = pack2<VT>(u.x, u.y);
             p[d + 1] = pack2<VT>(v.x, v.y);
           }
+        };
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t p[16];
+          if (MODE == kScaleToken && wild) weights(std::true_type{}, i, p);
+          else weights(std::false_type{}, i, p);
           tmem_st16(s_addr + 16 * i, p);
           if (i == 1) {  // the product with the first 64 tokens can start
             tmem_wait_st();
@@ -724,6 +738,16 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
         block = a.c.tables[pt.b * a.c.table_stride + page];
       };
       look_up(x.k0);
+      // its scales, fetched a conversion ahead of their use
+      float ks = 0.f, vs = 0.f;
+      auto look_scales = [&]() {
+        ks = vs = 0.f;
+        if (MODE == kScaleToken && off >= 0 && (uint32_t)block < (uint32_t)a.c.num_blocks) {
+          const int64_t at = ((int64_t)block * a.c.block_size + off) * a.c.kv_heads + x.head;
+          ks = a.c.k_scale[at];
+          vs = a.c.v_scale[at];
+        }
+      };
       // where the rows of tile k are, and what the softmax needs to know of them
       auto prepare = [&](int k) {
         const bool known = (uint32_t)block < (uint32_t)a.c.num_blocks, here = off >= 0 && known;
@@ -731,10 +755,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
         row_at[buf][lt] = here ? (uint32_t)block * block16 + (uint32_t)off * page16 + (uint32_t)x.head * head16 : 0xffffffffu;
         Info& in = info[inf.s];
         const uint32_t word = __ballot_sync(0xffffffffu, here);
-        float ks = 0.f, vs = 0.f;
         if constexpr (MODE == kScaleToken) {
-          const int64_t at = here ? ((int64_t)block * a.c.block_size + off) * a.c.kv_heads + x.head : 0;
-          if (here) { ks = a.c.k_scale[at]; vs = a.c.v_scale[at]; }
           const float top = warp_max(fabsf(vs) <= FLT_MAX ? fabsf(vs) : 0.f);
           const bool wild = __any_sync(0xffffffffu, !(fabsf(vs) <= FLT_MAX));
           const bool odd = __any_sync(0xffffffffu, !(ks >= 0.f && ks <= FLT_MAX));
@@ -842,12 +863,14 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
           }
           st.advance(ST);
         };
+        look_scales();
         prepare(x.k0);
         fetch(0);  // (Q is in the same group)
         fetch(1);
         for (int k = x.k0; k < x.k1 && ok; ++k) {
           const bool more = k + 1 < x.k1;
           asm volatile("cp.async.wait_group 1;" ::: "memory");
+          look_scales();
           convert(std::integral_constant<int, 0>{}, k == x.k0);
           if (!ok) break;
           buf ^= 1;
