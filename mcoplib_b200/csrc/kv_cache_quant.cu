@@ -9,88 +9,99 @@ namespace {
 // Store: per (token, head) row  s = max|x| / 127 (one IEEE fp32 division),  code = nearest integer of the REAL quotient
 // x / s, ties to even.  The quotient is never formed: n = rint(x * rn(1/s)) is off by one at most (|x * rn(1/s)| <= 127.5
 // and carries two roundings, 2^-16 in absolute terms), and the sign of the residual fma(-(n +- 1/2), s, x), which one rounding
-// cannot change, says on which side of the midpoint x lies.  Only lanes within 2^-12 of a midpoint look.
+// cannot change, says on which side of the midpoint x lies.  Only threads with an element within 2^-15 of a midpoint look.
 // A row of zeros has s = 0 and codes 0; a row that holds a NaN or an infinity has s = NaN and codes 0, so that it reads
 // back as NaN instead of as plausible values.
 //
-// Bound: HBM bytes (2 * head_size read, head_size + 4 written per row).  A row sits on LANES lanes of 16 elements: two
-// 16-byte loads and one 16-byte store per lane; a thread does one row slice, so 64 KB of loads are in flight per SM.
+// Bound: HBM bytes (2 * head_size read, head_size + 4 written per row).  A row sits on LANES lanes, each with 8 elements of its
+// first and 8 of its second half, so that every load and store of a warp covers whole sectors (16 neighbouring elements per
+// lane fetched each sector twice).
 // ---------------------------------------------------------------------------------------------
-template <typename T> __device__ __forceinline__ void load16(const T* p, float (&v)[16]) {
-  float a[8], b[8];
-  Vec8<T>::load_nc(p, a);
-  Vec8<T>::load_nc(p + 8, b);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) { v[i] = a[i]; v[8 + i] = b[i]; }
-}
-
-// Smallest normal scale for which 1/s is finite and the residuals are exact enough; smaller ones take the division.
+// Smallest scale for which 1/s is finite and the residuals are exact enough; smaller ones take the division.
 constexpr float kTinyScale = 0x1p-100f;
-
-__device__ __forceinline__ int nearest_code(float x, float s, float inv) {
-  float n;
-  if (s < kTinyScale) {  // subnormal territory (1/s may overflow): the quotient in double is exact enough to round once
-    n = (float)rint((double)x / (double)s);
-  } else {
-    const float t = __fmul_rn(x, inv);
-    n = rintf(t);
-    if (fabsf(__fsub_rn(t, n)) > 0.5f - 0x1p-12f) {
-      const float up = __fmaf_rn(-(n + 0.5f), s, x), down = __fmaf_rn(-(n - 0.5f), s, x);
-      const bool odd = ((int)n) & 1;
-      if (up > 0.f || (up == 0.f && odd)) n += 1.f;
-      else if (down < 0.f || (down == 0.f && odd)) n -= 1.f;
-    }
-  }
-  return max(-127, min(127, (int)n));
-}
 
 template <typename T, int LANES>
 __global__ void __launch_bounds__(256) kv_quant_store_kernel(const T* __restrict__ key, const T* __restrict__ value, int64_t key_stride,
                                                              int64_t value_stride, int8_t* __restrict__ key_cache,
                                                              int8_t* __restrict__ value_cache, int64_t block_stride, int64_t page_stride,
                                                              int64_t head_stride, float* __restrict__ k_scale, float* __restrict__ v_scale,
-                                                             const int64_t* __restrict__ slots, int64_t rows, int kv_heads, int head_size,
-                                                             int block_size, int64_t capacity, int* err) {
+                                                             const int64_t* __restrict__ slots, uint32_t rows, uint32_t kv_heads, int head_size,
+                                                             uint32_t block_size, int64_t capacity, Divisor by_rows, Divisor by_block, int* err) {
   pdl_launch_dependents();
   pdl_wait();
-  const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LANES;  // (token, K or V, head)
-  const int lane = threadIdx.x % LANES, d0 = lane * 16;
-  const bool live = row < rows && d0 < head_size;
-  const int64_t token = row / (2 * kv_heads);
-  const int rest = (int)(row - token * (2 * kv_heads));
+  const uint32_t row = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;  // (token, K or V, head)
+  const int lane = threadIdx.x % LANES, d0 = lane * 8, d1 = d0 + LANES * 8;
+  const bool live = row < rows;
+  const uint32_t token = live ? by_rows.of(row) : 0, rest = row - token * (2 * kv_heads);
   const bool is_v = rest >= kv_heads;
-  const int head = is_v ? rest - kv_heads : rest;
-  const int64_t slot = row < rows ? slots[token] : -1;
+  const uint32_t head = is_v ? rest - kv_heads : rest;
+  const int64_t slot = live ? slots[token] : -1;
   float x[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) x[i] = 0.f;
-  if (live) load16((is_v ? value + token * value_stride : key + token * key_stride) + head * head_size + d0, x);
-  float m = 0.f;
-  bool bad = false;
+  if (live) {
+    const T* p = (is_v ? value + token * value_stride : key + token * key_stride) + head * head_size;
+    float a[8], b[8];
+    if (d0 < head_size) {
+      Vec8<T>::load_nc(p + d0, a);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    m = fmaxf(m, fabsf(x[i]));
-    bad |= !(fabsf(x[i]) <= FLT_MAX);
+      for (int i = 0; i < 8; ++i) x[i] = a[i];
+    }
+    if (d1 < head_size) {
+      Vec8<T>::load_nc(p + d1, b);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[8 + i] = b[i];
+    }
   }
-  if (bad) m = INFINITY;
+  float m = 0.f;  // a NaN stays one
 #pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  for (int i = 0; i < 16; i += 2) asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(x[i]), "f"(x[i + 1]));
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) {
+    const float other = __shfl_xor_sync(0xffffffffu, m, o);
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(other));
+  }
   if (!live || slot < 0) return;
   if (slot >= capacity) {
     if (lane == 0) report(err, MCOP_DEVERR_SLOT);
     return;
   }
-  const int64_t block = slot / block_size;
-  const int64_t at = block * block_stride + (slot - block * block_size) * page_stride + head * head_stride + d0;
+  const uint32_t block = by_block.of((uint32_t)slot);
+  int8_t* out = (is_v ? value_cache : key_cache) + block * block_stride + ((uint32_t)slot - block * block_size) * page_stride + head * head_stride;
   const bool finite = m <= FLT_MAX;
   const float s = finite ? __fdiv_rn(m, 127.f) : __int_as_float(0x7fc00000);
-  uint32_t w[4] = {0, 0, 0, 0};
-  if (finite && s > 0.f) {
-    const float inv = __frcp_rn(s);
+  uint32_t q[16];
+  const float inv = finite && s > 0.f ? __frcp_rn(s) : 0.f;
+  const float2 inv2 = make_float2(inv, inv);
+  float far = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) w[i / 4] |= (uint32_t)(nearest_code(x[i], s, inv) & 0xff) << (8 * (i % 4));
+  for (int i = 0; i < 16; i += 2) {
+    // 1.5 * 2^23: the low byte of the sum is x * inv rounded to an integer, ties to even
+    const float2 v = make_float2(x[i], x[i + 1]), u = __ffma2_rn(v, inv2, make_float2(12582912.f, 12582912.f));
+    const float2 minus_n = __ffma2_rn(u, make_float2(-1.f, -1.f), make_float2(12582912.f, 12582912.f)), d = __ffma2_rn(v, inv2, minus_n);
+    q[i] = __float_as_uint(u.x);
+    q[i + 1] = __float_as_uint(u.y);
+    far = max3_abs(far, d.x, d.y);
   }
-  st_u4((is_v ? value_cache : key_cache) + at, make_uint4(w[0], w[1], w[2], w[3]));
+  if (finite && s > 0.f) {
+    if (s < kTinyScale) {  // subnormal territory (1/s may overflow): the quotient in double is exact enough to round once
+#pragma unroll
+      for (int i = 0; i < 16; ++i) q[i] = (uint32_t)max(-127, min(127, (int)rint((double)x[i] / (double)s)));
+    } else if (far > 0.5f - 0x1p-15f) {  // (half of the largest value is the midpoint 63.5: common, so this is branch-free)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float n = __fsub_rn(__uint_as_float(q[i]), 12582912.f), d = __fmaf_rn(x[i], inv, -n);
+        const float beyond = copysignf(1.f, d), r = __fmaf_rn(-__fmaf_rn(0.5f, beyond, n), s, x[i]) * beyond;
+        if (r > 0.f || (r == 0.f && (q[i] & 1))) q[i] += d < 0.f ? ~0u : 1u;
+      }
+    }
+  }
+  if (!finite) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) q[i] = 0;
+  }
+  if (d0 < head_size) *reinterpret_cast<uint2*>(out + d0) = make_uint2(pack4_low_bytes(q[0], q[1], q[2], q[3]), pack4_low_bytes(q[4], q[5], q[6], q[7]));
+  if (d1 < head_size) *reinterpret_cast<uint2*>(out + d1) = make_uint2(pack4_low_bytes(q[8], q[9], q[10], q[11]), pack4_low_bytes(q[12], q[13], q[14], q[15]));
   if (lane == 0) (is_v ? v_scale : k_scale)[slot * kv_heads + head] = s;
 }
 
@@ -123,30 +134,51 @@ __global__ void __launch_bounds__(256) kv_gather_kernel(T* __restrict__ key_out,
   }
   const int64_t off = pos - page * c.block_size;
   const int64_t base = block * c.block_stride + off * c.page_stride, slot = block * c.block_size + off;
-  const int per_head = head_size / 16, chunks = c.kv_heads * per_head;
-  const int64_t out0 = t * (int64_t)c.kv_heads * head_size;
-  for (int i = lane; i < 2 * chunks; i += 32) {
-    const bool is_v = i >= chunks;
-    const int j = is_v ? i - chunks : i;
-    const int head = j / per_head, d0 = (j - head * per_head) * 16;
-    const int64_t at = base + head * c.head_stride + d0;
-    T* o = (is_v ? value_out : key_out) + out0 + j * 16;
-    if constexpr (I8) {
-      const uint4 u = ld_nc_u4(static_cast<const int8_t*>(is_v ? c.v : c.k) + at);
-      const float* sp = is_v ? c.v_scale : c.k_scale;
-      const float s = scale_mode == kScaleToken ? sp[slot * c.kv_heads + head] : sp[head];
-      float v[8], w[8];
-      unpack_i8x8(make_uint2(u.x, u.y), v);
-      unpack_i8x8(make_uint2(u.z, u.w), w);
+  // pieces of 8 elements, 4 to 8 of them in flight per lane: every load and store of the warp covers whole sectors
+  const int per_head = head_size / 8, pieces = c.kv_heads * per_head;
+  const int64_t out0 = t * (int64_t)pieces * 8;
+  constexpr int N = 4;
+  for (int i0 = lane; i0 < pieces; i0 += 32 * N) {
+    uint2 k8[N], v8[N];
+    uint4 k16[N], v16[N];
+    float ks[N], vs[N];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) { v[k] = __fmul_rn(v[k], s); w[k] = __fmul_rn(w[k], s); }
-      Vec8<T>::store(o, v);
-      Vec8<T>::store(o + 8, w);
-    } else {
-      const T* p = static_cast<const T*>(is_v ? c.v : c.k) + at;
-      const uint4 u = ld_nc_u4(p), w = ld_nc_u4(p + 8);
-      st_u4(o, u);
-      st_u4(o + 8, w);
+    for (int n = 0; n < N; ++n) {
+      const int i = i0 + 32 * n;
+      if (i < pieces) {
+        const int head = i / per_head;
+        const int64_t at = base + head * c.head_stride + (i - head * per_head) * 8;
+        if constexpr (I8) {
+          k8[n] = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(c.k) + at);
+          v8[n] = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(c.v) + at);
+          const int64_t si = scale_mode == kScaleToken ? slot * c.kv_heads + head : head;
+          ks[n] = c.k_scale[si];
+          vs[n] = c.v_scale[si];
+        } else {
+          k16[n] = ld_nc_u4(static_cast<const T*>(c.k) + at);
+          v16[n] = ld_nc_u4(static_cast<const T*>(c.v) + at);
+        }
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int i = i0 + 32 * n;
+      if (i < pieces) {
+        if constexpr (I8) {
+          float v[8];
+          unpack_i8x8(k8[n], v);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(v[j], ks[n]);
+          Vec8<T>::store(key_out + out0 + i * 8, v);
+          unpack_i8x8(v8[n], v);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(v[j], vs[n]);
+          Vec8<T>::store(value_out + out0 + i * 8, v);
+        } else {
+          st_u4(key_out + out0 + i * 8, k16[n]);
+          st_u4(value_out + out0 + i * 8, v16[n]);
+        }
+      }
     }
   }
 }
@@ -158,11 +190,12 @@ int launch_store(const void* key, const void* value, int64_t ks, int64_t vs, int
   const int64_t rows = tokens * 2 * kv_heads;
   int lanes = 1;
   while (lanes * 16 < head_size) lanes *= 2;
+  MCOP_REQUIRE(rows < INT32_MAX / 2, MCOP_ERR_UNSUPPORTED, "reshape_and_cache_dynamic_int8: too many rows");
   const int64_t ctas = (rows * lanes + 255) / 256;
-  MCOP_REQUIRE(ctas <= INT32_MAX, MCOP_ERR_UNSUPPORTED, "reshape_and_cache_dynamic_int8: too many rows");
   auto go = [&](auto kernel) {
     launch_pdl(kernel, dim3((unsigned)ctas), dim3(256), 0, st, static_cast<const T*>(key), static_cast<const T*>(value), ks, vs, kc, vc, bs,
-               ps, hs, k_scale, v_scale, slots, rows, kv_heads, head_size, block_size, num_blocks * block_size, pipe_error_ptr());
+               ps, hs, k_scale, v_scale, slots, (uint32_t)rows, (uint32_t)kv_heads, head_size, (uint32_t)block_size, num_blocks * block_size,
+               Divisor(2u * (uint32_t)kv_heads), Divisor((uint32_t)block_size), pipe_error_ptr());
     return check_launch("reshape_and_cache_dynamic_int8");
   };
   switch (lanes) {

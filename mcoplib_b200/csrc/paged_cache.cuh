@@ -11,6 +11,18 @@ namespace mcop {
 
 enum ScaleMode { kScaleNone = 0, kScaleHead = 1, kScaleToken = 2 };
 
+// Division of p < 2^31 by a fixed d as a multiplication: with 2^(s-1) < d <= 2^s and m = ceil(2^(31 + s) / d) < 2^32,
+// floor(p * m / 2^(31 + s)) = floor(p / d), since m exceeds 2^(31 + s) / d by less than 2^s / d.
+struct Divisor {
+  uint32_t mul = 0, shift = 0;
+  Divisor() = default;
+  __host__ explicit Divisor(uint32_t d) {
+    while ((uint64_t(1) << shift) < d) ++shift;
+    mul = (uint32_t)(((uint64_t(1) << (31 + shift)) + d - 1) / d);
+  }
+  __device__ __forceinline__ uint32_t of(uint32_t p) const { return __umulhi(2u * p, mul) >> shift; }
+};
+
 struct PagedCache {
   const void* k;
   const void* v;
@@ -23,15 +35,10 @@ struct PagedCache {
   int block_size;
   int64_t num_blocks;
   int kv_heads;
-  uint32_t page_mul = 0, page_shift = 0;
+  Divisor by_block;  // the division by block_size
 
-  // The division by the block size as a multiplication: with 2^(s-1) < d <= 2^s and m = ceil(2^(31 + s) / d) < 2^32,
-  // floor(p * m / 2^(31 + s)) = floor(p / d) for every p < 2^31 (m exceeds 2^(31 + s) / d by less than 2^s / d).
-  __host__ void prepare() {
-    while ((int64_t(1) << page_shift) < block_size) ++page_shift;
-    page_mul = (uint32_t)(((uint64_t(1) << (31 + page_shift)) + block_size - 1) / block_size);
-  }
-  __device__ __forceinline__ int page_of(int p) const { return (int)(__umulhi(2u * (uint32_t)p, page_mul) >> page_shift); }
+  __host__ void prepare() { by_block = Divisor((uint32_t)block_size); }
+  __device__ __forceinline__ int page_of(int p) const { return (int)by_block.of((uint32_t)p); }
 };
 
 __device__ __forceinline__ void report(int* err, int code) {
