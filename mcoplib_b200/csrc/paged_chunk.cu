@@ -992,8 +992,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
 }
 
 // Joins the partial results of the items that cross CTA borders: CTA c of the kernel above holds the first part of at most one such
-// item, the CTAs behind it one part each.  blockIdx.y: 32 rows; a thread takes four elements of one row at a time.
-template <typename T, int DP> __global__ void __launch_bounds__(256) chunk_join_kernel(AttnArgs a, Layout w) {
+// item, the CTAs behind it one part each.  blockIdx.y: 16 rows; a thread takes four elements of one row at a time.
+template <typename T, int DP> __global__ void __launch_bounds__(512) chunk_join_kernel(AttnArgs a, Layout w) {
   pdl_launch_dependents();
   pdl_wait();
   const Rec rec = w.recs[blockIdx.x];
@@ -1001,8 +1001,8 @@ template <typename T, int DP> __global__ void __launch_bounds__(256) chunk_join_
   const int G = a.q_heads / a.c.kv_heads, d = threadIdx.x % (DP / 4) * 4;
   const Seq s = sequence(a, rec.b);
   auto part = [&](int i) { return w.parts + (int64_t)(i == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + i)) * (kRows * (DP + 2)); };
-  for (int i = threadIdx.x / (DP / 4); i < 32; i += 1024 / DP) {
-    const int row = blockIdx.y * 32 + i, flat = rec.t * kRows + row, token = flat / G, head = rec.head * G + flat - token * G;
+  for (int i = threadIdx.x / (DP / 4); i < 16; i += 2048 / DP) {
+    const int row = blockIdx.y * 16 + i, flat = rec.t * kRows + row, token = flat / G, head = rec.head * G + flat - token * G;
     if (token >= s.qn) return;
     float top = -INFINITY;
 #pragma unroll 4
@@ -1041,7 +1041,7 @@ template <typename T, int MODE, int DP> int launch_one(const AttnArgs& a, void* 
   if (int rc = check_launch(what)) return rc;
   launch_pdl(kernel, dim3(grid), dim3(kThreads), C::SMEM, st, a, w);
   if (int rc = check_launch(what)) return rc;
-  launch_pdl(chunk_join_kernel<T, DP>, dim3(grid, kRows / 32), dim3(256), 0, st, a, w);
+  launch_pdl(chunk_join_kernel<T, DP>, dim3(grid, kRows / 16), dim3(512), 0, st, a, w);
   return check_launch(what);
 }
 

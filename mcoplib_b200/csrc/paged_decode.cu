@@ -582,28 +582,41 @@ __global__ void __launch_bounds__(kThreads, Cfg<T, MODE, DP, NT>::CTAS) decode_k
 }
 
 // Joins the partial results of the items that cross CTA borders: CTA c of the kernel above holds the first part of at most
-// one such item, the CTAs behind it one part each.  A thread takes four elements of one head.
+// one such item, the CTAs behind it one part each.  A thread takes four elements of one head, and every GROUPS-th part: the parts
+// come from L2, and it is the number of loads on their way that counts (one long sequence has 16 parts or more per head).
+template <int DP, int NT> struct Join {
+  static constexpr int SPAN = 2 * NT * DP;               // threads that cover all heads of an item
+  static constexpr int GROUPS = SPAN <= 256 ? 4 : 2;
+};
 template <typename T, int MODE, int DP, int NT>
-__global__ void __launch_bounds__(2 * NT * DP) decode_join_kernel(AttnArgs a, const float* __restrict__ parts, const Rec* __restrict__ recs) {
+__global__ void __launch_bounds__(Join<DP, NT>::SPAN * Join<DP, NT>::GROUPS) decode_join_kernel(AttnArgs a, const float* __restrict__ parts,
+                                                                                               const Rec* __restrict__ recs) {
   using C = Cfg<T, MODE, DP, NT>;
+  using J = Join<DP, NT>;
+  __shared__ int tops[C::HEADS];
+  __shared__ float4 part_x[J::GROUPS - 1][J::SPAN];
+  __shared__ float part_sum[J::GROUPS - 1][J::SPAN];
   pdl_launch_dependents();
   pdl_wait();
   const Rec r = recs[blockIdx.x];
   if (r.count == 0) return;
   const int G = a.q_heads / a.c.kv_heads, head_tiles = (G + C::HEADS - 1) / C::HEADS;
-  const int hh = threadIdx.x / (DP / 4), d = threadIdx.x % (DP / 4) * 4;
-  const int kv_head = r.tile / head_tiles, h = (r.tile - kv_head * head_tiles) * C::HEADS + hh;
-  if (h >= G) return;
-  const Seq s = sequence(a, r.b);
-  auto part = [&](int i) { return parts + (int64_t)(i == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + i)) * C::SLOT; };
-  float top = -INFINITY;
-#pragma unroll 4
-  for (int i = 0; i < r.count; ++i) top = fmaxf(top, part(i)[C::HEADS * DP + 2 * hh]);
-  const float safe = top == -INFINITY ? 0.f : top;
+  const int group = threadIdx.x / J::SPAN, me = threadIdx.x % J::SPAN, hh = me / (DP / 4), d = me % (DP / 4) * 4;
+  auto part = [&](int i) { return parts + (int64_t)(2 * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * C::SLOT; };
+  // the largest maximum of each head, as an integer of the same order
+  auto ordered = [](float x) { const int i = __float_as_int(x); return i < 0 ? i ^ 0x7fffffff : i; };
+  if (threadIdx.x < C::HEADS) tops[threadIdx.x] = ordered(-INFINITY);
+  __syncthreads();
+  int mine = ordered(-INFINITY);
+  for (int i = group * (DP / 4) + me % (DP / 4); i < r.count; i += J::GROUPS * (DP / 4)) mine = max(mine, ordered(part(i)[C::HEADS * DP + 2 * hh]));
+  if (mine != ordered(-INFINITY)) atomicMax(&tops[hh], mine);
+  __syncthreads();
+  const int ti = tops[hh];
+  const float top = __int_as_float(ti < 0 ? ti ^ 0x7fffffff : ti), safe = top == -INFINITY ? 0.f : top;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
   float sum = 0.f;
 #pragma unroll 4
-  for (int i = 0; i < r.count; ++i) {
+  for (int i = group; i < r.count; i += J::GROUPS) {
     const float2 ml = *reinterpret_cast<const float2*>(part(i) + C::HEADS * DP + 2 * hh);
     const float4 v = *reinterpret_cast<const float4*>(part(i) + hh * DP + d);
     const float w = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2_approx(ml.x - safe);
@@ -613,14 +626,27 @@ __global__ void __launch_bounds__(2 * NT * DP) decode_join_kernel(AttnArgs a, co
     x.z = __fmaf_rn(w, v.z, x.z);
     x.w = __fmaf_rn(w, v.w, x.w);
   }
-  if (s.qn == 0) return;
+  if (group > 0) {
+    part_x[group - 1][me] = x;
+    part_sum[group - 1][me] = sum;
+  }
+  __syncthreads();
+  if (group > 0) return;
+#pragma unroll
+  for (int g = 0; g < J::GROUPS - 1; ++g) {
+    const float4 y = part_x[g][me];
+    x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+    sum += part_sum[g][me];
+  }
+  const int kv_head = r.tile / head_tiles, h = (r.tile - kv_head * head_tiles) * C::HEADS + hh;
+  if (h >= G) return;
   float f = sum == 0.f ? 0.f : 1.f / sum;
   if (MODE == kScaleHead) f *= a.c.v_scale[kv_head];
   const int head = kv_head * G + h;
   if (d < a.head_size)
-    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (int64_t)s.q0 * a.o_token + (int64_t)head * a.o_head + d) =
+    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (int64_t)r.b * a.o_token + (int64_t)head * a.o_head + d) =
         make_uint2(pack2<T>(x.x * f, x.y * f), pack2<T>(x.z * f, x.w * f));
-  if (a.lse && d == 0) a.lse[(int64_t)s.q0 * a.q_heads + head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+  if (a.lse && d == 0) a.lse[(int64_t)r.b * a.q_heads + head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
 template <typename T, int MODE, int DP, int NT, bool FULL> int launch_one(const AttnArgs& a, void* ws, cudaStream_t st) {
@@ -633,7 +659,7 @@ template <typename T, int MODE, int DP, int NT, bool FULL> int launch_one(const 
   Rec* recs = reinterpret_cast<Rec*>(parts + (int64_t)grid * 2 * C::SLOT);
   launch_pdl(kernel, dim3(grid), dim3(kThreads), C::SMEM, st, a, parts, recs);
   if (int rc = check_launch("paged_attention_decode")) return rc;
-  launch_pdl(decode_join_kernel<T, MODE, DP, NT>, dim3(grid), dim3(2 * NT * DP), 0, st, a, (const float*)parts, (const Rec*)recs);
+  launch_pdl(decode_join_kernel<T, MODE, DP, NT>, dim3(grid), dim3(Join<DP, NT>::SPAN * Join<DP, NT>::GROUPS), 0, st, a, (const float*)parts, (const Rec*)recs);
   return check_launch("paged_attention_decode");
 }
 
