@@ -385,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
       float m = -INFINITY, l = 0.f;
       int e = -1000;
       if (idle) {  // no rows: keep in step with the item
-        if (!(ok = mbar_wait_bounded(&bars.o_full[group], o_phase, a.err, kWaitSoftmax, kSpin))) break;
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&bars.o_full[group], o_phase, a.err, kWaitSoftmax, kSpin)))) break;
         o_phase ^= 1;
         for (int k = x.k0; k < x.k1; ++k) inf.advance(C::NI);
         __syncwarp();
@@ -395,9 +395,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
       }
       for (int k = x.k0; k < x.k1 && ok; ++k) {
         const Info& in = info[inf.s];
-        if (!(ok = mbar_wait_bounded(&bars.info_full[inf.s], inf.phase, a.err, kWaitSoftmax, kSpin))) break;
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&bars.info_full[inf.s], inf.phase, a.err, kWaitSoftmax, kSpin)))) break;
         inf.advance(C::NI);
-        if (!(ok = mbar_wait_bounded(&bars.s_full[group], s_phase, a.err, kWaitSoftmax, kSpin))) break;
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&bars.s_full[group], s_phase, a.err, kWaitSoftmax, kSpin)))) break;
         s_phase ^= 1;
         tc_fence_after();
         float s[128];
@@ -545,7 +545,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
       }
       if (ok) {
         // O of the item
-        if (!(ok = mbar_wait_bounded(&bars.o_full[group], o_phase, a.err, kWaitSoftmax, kSpin))) break;
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&bars.o_full[group], o_phase, a.err, kWaitSoftmax, kSpin)))) break;
         o_phase ^= 1;
         tc_fence_after();
         const bool whole = x.k1 - x.k0 == pt.n;
@@ -642,6 +642,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
     int pending = 0;          // copies issued and not handed over (float caches)
     uint32_t with_q = 0, scan_v = 0;  // one bit per pending copy, the oldest in bit pending - 1: Q came with it; V of a masked tile
     uint32_t scan_item = 0;
+    // Once a wait has run out (ok false) a warp copies nothing more, but walks on to the end: the four meet at barriers.
     bool ok = true;
     int item = 0, buf = 0;
 
@@ -695,10 +696,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
         }
         hand_over();
       }
-      return mbar_wait_bounded(bar, phase, a.err, kWaitLoad, kSpin);
+      return __all_sync(0xffffffffu, mbar_wait_bounded(bar, phase, a.err, kWaitLoad, kSpin));
     };
 
-    while (ok && x.next(w, a.c.kv_heads, pt)) {
+    while (x.next(w, a.c.kv_heads, pt)) {
       if (lt == 0) *(volatile int*)&poison[item & 7] = 0;
       // rows of Q
       const Seq seq{pt.q0, pt.qn, pt.len};
@@ -708,11 +709,11 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
         q_at[row] = row < pt.rows ? (uint32_t)(((int64_t)(seq.q0 + token) * a.q_token + (int64_t)(x.head * G + flat - token * G) * a.q_head) / 8) : 0xffffffffu;
       }
       if (item > 0) {
-        if (!(ok = acquire(&bars.q_empty, q_phase))) break;
+        ok = ok && acquire(&bars.q_empty, q_phase);
         q_phase ^= 1;
       }
       sync();
-      {
+      if (ok) {
         const int c = lt % C::PIECES;
         for (int row = lt / C::PIECES; row < (pt.rows + 127) / 128 * 128; row += 128 / C::PIECES) {
           const uint32_t at = q_at[row];
@@ -798,14 +799,15 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
         look_up(k + 1);
       };
       if constexpr (!C::I8) {
-        for (int k = x.k0; k < x.k1 && ok; ++k) {
+        for (int k = x.k0; k < x.k1; ++k) {
           prepare(k);
           const int base = (pt.first + k) * kTile;
           const bool scan = base < all_lo || base + kTile > all_hi;
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
             const char* src = kv ? vbase : kbase;
-            if (!(ok = acquire(&bars.empty[st.s], st.phase ^ 1))) break;
+            ok = ok && acquire(&bars.empty[st.s], st.phase ^ 1);
+            if (!ok) continue;
             const uint32_t dst = ring + st.s * C::TILE;
             const int c = lt % C::PIECES;
 #pragma unroll
@@ -836,7 +838,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
         };
         auto convert = [&](auto which, bool with_q) {
           constexpr int kv = decltype(which)::value;
-          if (!(ok = mbar_wait_bounded(&bars.empty[st.s], st.phase ^ 1, a.err, kWaitLoad, kSpin))) return;
+          ok = ok && acquire(&bars.empty[st.s], st.phase ^ 1);
+          if (!ok) return;
           const uint32_t dst = ring + st.s * C::TILE, from = rawbuf + kv * (kTile * DP) + lt * 16;
 #pragma unroll
           for (int i = 0; i < N; ++i) {
@@ -865,18 +868,19 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
         };
         look_scales();
         prepare(x.k0);
-        fetch(0);  // (Q is in the same group)
-        fetch(1);
-        for (int k = x.k0; k < x.k1 && ok; ++k) {
+        if (ok) {
+          fetch(0);  // (Q is in the same group)
+          fetch(1);
+        }
+        for (int k = x.k0; k < x.k1; ++k) {
           const bool more = k + 1 < x.k1;
           asm volatile("cp.async.wait_group 1;" ::: "memory");
           look_scales();
           convert(std::integral_constant<int, 0>{}, k == x.k0);
-          if (!ok) break;
           buf ^= 1;
           if (more) {
             prepare(k + 1);
-            fetch(0);
+            if (ok) fetch(0);
             asm volatile("cp.async.wait_group 1;" ::: "memory");
           } else {
             asm volatile("cp.async.wait_group 0;" ::: "memory");

@@ -21,8 +21,6 @@ namespace {
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kMaxCtasPerSm = 3;
-// Fewer units than this per CTA are not worth a CTA's set-up and a partial result of their own.
-constexpr int kMinUnits = 2;
 
 struct Rec {
   int b, tile, count, pad;
@@ -167,7 +165,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<T, MODE, DP, NT>::CTAS) decode_k
     if (w < warp) incl += scan[w];
     total += scan[w];
   }
-  const int64_t per = max((int64_t)kMinUnits, (total + gridDim.x - 1) / gridDim.x);
+  const int64_t per = (total + gridDim.x - 1) / gridDim.x;
   const int64_t u0 = per * blockIdx.x, u1 = min(total, u0 + per);
   if (u0 >= u1) {  // nothing left for this CTA
     if (tid == 0) recs[blockIdx.x].count = 0;
@@ -252,7 +250,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<T, MODE, DP, NT>::CTAS) decode_k
   auto fetch_k = [&](int st) {
     there = 0;
     if (in.u < units) {
-      const int kv_head = in.tile / head_tiles;
+      const int kv_head = head_tiles == 1 ? in.tile : in.tile / head_tiles;
       const bool known = (uint32_t)block < (uint32_t)a.c.num_blocks, here = off >= 0 && known;
       if (off >= 0 && !known) report(a.err, MCOP_DEVERR_SLOT);
       // a token that is not there is copied as zeros: nothing is read for it (reading some other row in its place made that row's
@@ -302,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<T, MODE, DP, NT>::CTAS) decode_k
   bool began_here = cur.k == 0;
 
   for (int u = 0; u < units; ++u) {
-    const int kv_head = cur.tile / head_tiles, h0 = (cur.tile - kv_head * head_tiles) * C::HEADS;
+    const int kv_head = head_tiles == 1 ? cur.tile : cur.tile / head_tiles, h0 = (cur.tile - kv_head * head_tiles) * C::HEADS;
     if (fresh) {
       fresh = false;
       const Seq s = sequence(a, cur.b);
