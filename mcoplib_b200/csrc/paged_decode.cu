@@ -407,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<T, MODE, DP, NT>::CTAS) decode_k
             ks = scales[tok];
             vs[hf][r] = scales[C::TOK + tok];
             // what a token's scale adds to its logit where the maximum is concerned (bounded, so that fp32 holds the weights' sum)
-            ref[hf][r] = __log2f(fminf(fmaxf(vs[hf][r], 0x1p-60f), 0x1p60f));
+            ref[hf][r] = __log2f(fminf(fmaxf(fabsf(vs[hf][r]), 0x1p-60f), 0x1p60f));
           }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {

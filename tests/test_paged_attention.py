@@ -302,3 +302,70 @@ def test_two_calls_at_once_on_two_streams(op):
     torch.cuda.synchronize()
     for oc, od in outs:
         assert torch.equal(oc, want_c) and torch.equal(od, want_d)
+
+
+@pytest.mark.parametrize("decode", [True, False])
+@pytest.mark.parametrize("rising", [True, False])
+def test_token_scales_over_a_wide_range(op, decode, rising):
+    """V scales over 2^13 along the positions (the reference of the weights has to follow), K scales over a factor of 16."""
+    new, total, D = ([1] if decode else [150]), [700], 128
+    c = make_cache(total, 2, D, 16, "token", torch.bfloat16, poison=False)
+    at = torch.arange(700, device=DEV)
+    page, off = c["tables"][0].long()[at // 16], at % 16
+    power = torch.linspace(-6, 7, 700, device=DEV) * (1 if rising else -1)
+    c["vs"][page, off] = (2.0 ** power)[:, None] * 0.03
+    c["ks"][page, off] *= 2.0 ** torch.randint(-2, 3, (700, 1), device=DEV)
+    q = torch.randn(sum(new), 8, D, device=DEV).bfloat16()
+    out, lse = torch.empty_like(q), torch.empty(sum(new), 8, device=DEV)
+    if decode:
+        op.paged_attention_decode(out, q, c["k"], c["v"], c["tables"], lengths(total), 0.1, c["ks"], c["vs"], 0, lse)
+    else:
+        op.paged_attention_chunk(out, q, c["k"], c["v"], c["tables"], lengths(total), bounds(new), 0.1, c["ks"], c["vs"], True, 0, lse)
+    ref, rlse, spread, mass, reach = P.attention(q, c["k"], c["v"], c["tables"], torch.tensor(total), bounds(new).tolist(), 0.1, c["ks"], c["vs"])
+    tol, ltol = attention_tolerance(ref, rlse, spread, mass, reach, D, "token", torch.bfloat16)
+    # f16 holds weight * scale relative to a power of two that is at most twice the largest scale seen: below 2^-14 of it the
+    # rounding is absolute, 2^-25, times |code|
+    codes = c["v"][page, off].abs().double().sum(0).repeat_interleave(4, 0)
+    tol = tol + 2.0 ** -24 * float(c["vs"][page, off].max()) * codes
+    compare(out, ref, tol, "out")
+    compare(lse, rlse, ltol, "lse")
+
+
+@pytest.mark.parametrize("decode", [True, False])
+@pytest.mark.parametrize("kind", ["head", "token"])
+def test_negative_and_zero_scales(op, decode, kind):
+    new, total, D = ([1, 1] if decode else [90, 3]), [300, 40], 128
+    c = make_cache(total, 3, D, 16, kind, torch.bfloat16, poison=False)
+    c["ks"][..., 0] *= -1
+    c["ks"][..., 1] = 0
+    c["vs"][..., 2] *= -1
+    if kind == "token":
+        c["vs"][:, ::3, 1] = 0
+    q = torch.randn(sum(new), 6, D, device=DEV).bfloat16()
+    out, lse = torch.empty_like(q), torch.empty(sum(new), 6, device=DEV)
+    if decode:
+        op.paged_attention_decode(out, q, c["k"], c["v"], c["tables"], lengths(total), 0.1, c["ks"], c["vs"], 0, lse)
+    else:
+        op.paged_attention_chunk(out, q, c["k"], c["v"], c["tables"], lengths(total), bounds(new), 0.1, c["ks"], c["vs"], True, 0, lse)
+    _check(out, lse, q, c, total, bounds(new), 0.1, kind)
+
+
+def test_more_sequences_and_more_tiles_than_a_pass_of_the_plan(op):
+    """Over 1024 sequences, and one sequence of over 1024 query tiles."""
+    total = [1 + i % 3 for i in range(2100)]
+    c = make_cache(total, 1, 64, 2, "head", torch.bfloat16)
+    new = [0 if i % 7 == 3 else 1 for i in range(2100)]
+    q = torch.randn(sum(new), 2, 64, device=DEV).bfloat16()
+    out, lse = torch.empty_like(q), torch.empty(sum(new), 2, device=DEV)
+    op.paged_attention_chunk(out, q, c["k"], c["v"], c["tables"], lengths(total), bounds(new), 0.1, c["ks"], c["vs"], True, 0, lse)
+    _check(out, lse, q, c, total, bounds(new), 0.1, "head")
+    n = 40000
+    c = make_cache([n], 1, 64, 64, "float", torch.bfloat16)
+    q = torch.randn(n, 8, 64, device=DEV).bfloat16()
+    out, lse = torch.empty_like(q), torch.empty(n, 8, device=DEV)
+    op.paged_attention_chunk(out, q, c["k"], c["v"], c["tables"], lengths([n]), bounds([n]), 0.1, window=300, lse=lse)
+    for lo, hi in ((0, 60), (20000, 20060), (n - 60, n)):
+        ref, rlse, spread, mass, reach = P.attention(q[lo:hi], c["k"], c["v"], c["tables"], torch.tensor([hi]), [0, hi - lo], 0.1, window=300)
+        tol, ltol = attention_tolerance(ref, rlse, spread, mass, reach, 64, "float", torch.bfloat16)
+        compare(out[lo:hi], ref, tol, f"rows {lo}")
+        compare(lse[lo:hi], rlse, ltol, f"rows {lo} lse")
