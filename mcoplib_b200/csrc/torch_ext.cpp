@@ -463,7 +463,7 @@ int check_paged_cache(const Tensor& key_cache, const Tensor& value_cache, const 
                   stride_of(key_cache, 1) == stride_of(value_cache, 1) && stride_of(key_cache, 2) == stride_of(value_cache, 2) &&
                   key_cache.scalar_type() == value_cache.scalar_type(),
               "key_cache and value_cache must be [num_blocks, block_size, kv_heads, head_size] and share type and layout");
-  TORCH_CHECK(key_cache.stride(3) == 1, "the heads of the caches must be contiguous");
+  TORCH_CHECK(key_cache.stride(3) == 1 && value_cache.stride(3) == 1, "the heads of the caches must be contiguous");
   TORCH_CHECK(key_cache.device() == value_cache.device(), "the caches must be on one device");
   if (key_cache.scalar_type() != at::kChar) {
     TORCH_CHECK(key_cache.scalar_type() == type, "the cache must be int8 or of the type of the other tensors");
