@@ -281,9 +281,9 @@ int mcop_paged_attention_decode(void* out, int64_t out_token_stride, int64_t out
  * No counterpart in the reference.  query, out [tokens, q_heads, head_size]: rows cu_seqlens_q[b] .. cu_seqlens_q[b + 1] (int32 [batch + 1]) are
  * sequence b's last q_len tokens, so new token i stands at position pos = seq_lens[b] - q_len + i.  It sees the positions
  * j <= pos (causal != 0; otherwise all) with j > pos - window (window 0: no lower bound).  A token that sees nothing gets
- * out = 0 and lse = -inf.  Rows of out and lse outside the sequences keep what they held.  With a scale per token the weights
- * times the V scales are held in f16 relative to the largest scale so far: scales that differ by more than 2^14 within what a row
- * sees cost the rows that the smallest dominate some of their bits.  The rest as for decode. */
+ * out = 0 and lse = -inf.  Rows of out and lse outside the sequences keep what they held.  With a scale per token the products of
+ * weight and V scale are held in f16 relative to the largest weight times the largest scale among 128 tokens that the row sees: a
+ * product below 2^-14 of that loses bits.  What a row does not see changes nothing.  The rest as for decode. */
 size_t mcop_paged_attention_chunk_workspace_bytes(int64_t tokens, int batch, int q_heads, int kv_heads, int head_size);
 int mcop_paged_attention_chunk(void* out, int64_t out_token_stride, int64_t out_head_stride, float* lse, const void* query,
                                int64_t query_token_stride, int64_t query_head_stride, const void* key_cache,

@@ -271,16 +271,22 @@ struct Ring {
 };
 // What the softmax has to know of a tile's tokens beside the logits.
 struct alignas(16) TileInfo {
-  float ks[kTile], vs[kTile];  // kScaleToken: K scale times the logit factor, V scale times 2^-e
+  float ks[kTile], vs[kTile];  // kScaleToken: K scale times the logit factor, V scale
   uint32_t here[4];            // which tokens are there (their page is in the cache)
-  int all, e;                  // all of those inside the reach are; e of the V scales
+  int all;                     // all of those inside the reach are
+  float power;                 // scale_power of the largest finite V scale
   int wild, odd;               // a V scale is not finite; a K scale is not, or is negative
   float kmax, pad[3];          // the largest factor
 };
 struct TileBits {
   uint32_t here[4];
-  int all, e;
+  int all;
 };
+// With a scale per token the running maximum follows, tile by tile, the largest logit plus the power of two above the largest V
+// scale that the row sees there: weight times scale then lies below 2^kMaxSlack and fits f16.  Hidden tokens have no say: a tile's
+// own power would let them take bits from the rows of an item that do not see them.  Scales count within 2^-90 and 2^100, so that
+// fp32 holds the weights and their sum.
+__device__ __forceinline__ float scale_power(float largest) { return (float)min(100, max(-90, (int)(__float_as_uint(largest) >> 23) - 126)); }
 
 template <typename Info, int ST, int NI> struct Control {
   Info info[NI];
@@ -383,7 +389,6 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
       const bool flip = c < 0.f;  // a negative scale: the largest logit is the smallest product
       c = c == 0.f ? 1e-37f : fabsf(c);  // (0 times the -inf of a hidden column would be NaN)
       float m = -INFINITY, l = 0.f;
-      int e = -1000;
       if (idle) {  // no rows: keep in step with the item
         if (!(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&bars.o_full[group], o_phase, a.err, kWaitSoftmax, kSpin)))) break;
         o_phase ^= 1;
@@ -397,6 +402,12 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
         const Info& in = info[inf.s];
         if (!(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&bars.info_full[inf.s], inf.phase, a.err, kWaitSoftmax, kSpin)))) break;
         inf.advance(C::NI);
+        const int base = (pt.first + k) * kTile;
+        const bool masked = __any_sync(0xffffffffu, base < lo || base + kTile > hi) || !in.all;
+        auto seen_of = [&](int i) {  // columns [lo - base, hi - base) of [32 i, 32 i + 32) that are there
+          const int f = min(32, max(0, lo - base - 32 * i)), e = min(32, max(0, hi - base - 32 * i));
+          return (uint32_t)((1ull << e) - 1) & ~(uint32_t)((1ull << f) - 1) & in.here[i];
+        };
         if (!(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&bars.s_full[group], s_phase, a.err, kWaitSoftmax, kSpin)))) break;
         s_phase ^= 1;
         tc_fence_after();
@@ -410,8 +421,6 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
 #pragma unroll
           for (int i = 0; i < 128; ++i) s[i] = -s[i];
         }
-        const int base = (pt.first + k) * kTile;
-        const bool masked = __any_sync(0xffffffffu, base < lo || base + kTile > hi) || !in.all;
         // factors of the columns; where columns are hidden, the products with them are formed here
         uint32_t factor = 0, vfactor = 0;
         bool wild = false;
@@ -421,11 +430,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
           wild = in.wild;
         }
         if (masked) {
-          const int from = max(0, lo - base), to = hi - base;  // columns [from, to) are seen
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int f = min(32, max(0, from - 32 * i)), e = min(32, max(0, to - 32 * i));
-            const uint32_t seen = (uint32_t)((1ull << e) - 1) & ~(uint32_t)((1ull << f) - 1) & in.here[i];
+            const uint32_t seen = seen_of(i);
 #pragma unroll
             for (int d = 0; d < 32; ++d) {
               float v = s[32 * i + d];
@@ -441,11 +448,14 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
           for (int j = 0; j < 4; ++j) asm("max.f32 %0, %0, %1, %2;" : "+f"(tops[j]) : "f"(s[i + j]), "f"(s[i + j + 4]));
         }
         float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+        [[maybe_unused]] float logit = top;
         if constexpr (MODE == kScaleToken) {
           // The largest product, times the largest factor, bounds the logits; they are looked at one by one only where the
           // bound would move the maximum.
-          if (!masked) {
-            top = fmaxf(top, 0.f) * in.kmax;
+          if (masked) {
+            top += in.power;
+          } else {
+            top = fmaxf(top, 0.f) * in.kmax + in.power;
             if (__any_sync(0xffffffffu, top > m + kMaxSlack) || in.odd) {
               float2 best = make_float2(-INFINITY, -INFINITY);
 #pragma unroll
@@ -456,24 +466,35 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
                 asm("max.f32 %0, %0, %1, %2;" : "+f"(best.x) : "f"(u.x), "f"(u.y));
                 asm("max.f32 %0, %0, %1, %2;" : "+f"(best.y) : "f"(v.x), "f"(v.y));
               }
-              top = fmaxf(best.x, best.y);
+              top = fmaxf(best.x, best.y) + in.power;
             }
           }
         } else {
           top *= c;
         }
-        const bool grown = top > m + kMaxSlack;
-        const int e_new = in.e;
-        const bool moved = MODE == kScaleToken && e_new != e;
-        if (__any_sync(0xffffffffu, grown) || moved) {
+        bool grown = top > m + kMaxSlack;
+        if (__any_sync(0xffffffffu, grown)) {
+          if constexpr (MODE == kScaleToken) {
+            if (masked) {  // by what this row sees
+              float largest = 0.f;
+#pragma unroll 1
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t seen = seen_of(i);
+#pragma unroll
+                for (int d = 0; d < 32; d += 4) {
+                  const float4 f = lds4(vfactor + 128 * i + 4 * d);
+                  largest = fmaxf(fmaxf(largest, seen & 1u << d ? fabsf(f.x) : 0.f), seen & 2u << d ? fabsf(f.y) : 0.f);
+                  largest = fmaxf(fmaxf(largest, seen & 4u << d ? fabsf(f.z) : 0.f), seen & 8u << d ? fabsf(f.w) : 0.f);
+                }
+              }
+              top = logit + scale_power(largest);
+              grown = top > m + kMaxSlack;
+            }
+          }
           const float to = grown ? top : m;
           float keep = m == -INFINITY ? 0.f : exp2_approx(m - to);
           m = to;
           l *= keep;
-          if (moved) {
-            keep *= exp2_approx((float)max(-120, e - e_new));
-            e = e_new;
-          }
           if (k > x.k0) {
             // (S of this tile was issued behind the previous tile's P V: that product is complete)
 // (8 columns at a time: the logits stay in registers meanwhile)
@@ -491,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
         }
         const float safe = m == -INFINITY ? 0.f : m;
         float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
-        // 32 weights: rounded, summed, times their tokens' scales.  FIX: a scale that is not finite reaches only the rows that see its token.
+        // 32 weights: summed, times their tokens' scales, rounded.  FIX: a scale that is not finite reaches only the rows that see its token.
         auto weights = [&](auto FIX, int i, uint32_t* p) {
           const float2 shift = make_float2(-safe, -safe);
 #pragma unroll
@@ -550,7 +571,6 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
         tc_fence_after();
         const bool whole = x.k1 - x.k0 == pt.n;
         float f = 1.f;
-        if (MODE == kScaleToken) f = exp2_approx((float)e);
         if (MODE == kScaleHead) f = a.c.v_scale[x.head];
         const float norm = whole ? (l == 0.f ? 0.f : f / l) : f;
         float* part = w.parts + (int64_t)(2 * blockIdx.x + (x.k0 == 0 ? 1 : 0)) * (kRows * (DP + 2));
@@ -726,7 +746,6 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
       int all_lo, all_hi, other;
       span(a, seq, (pt.t * kRows + pt.rows - 1) / G, all_lo, other);
       span(a, seq, pt.t * kRows / G, other, all_hi);
-      int e = -1000;
       // page of token `lt` of a tile, fetched a tile ahead
       int block = -1, off = -1;
       auto look_up = [&](int k) {
@@ -781,17 +800,14 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
             in.wild = wild;
             in.odd = klow < 0.f;
             in.kmax = ktop * (a.scale * kLog2e) * (1.f + 0x1p-20f);
+            in.power = scale_power(top);
           }
-          // 2^e >= the tile's largest scale; moved only upwards and by more than 2^6, so that weight times scale stays below
-          // 2^14 (f16 ends at 2^16) and O is rescaled rarely
-          const int need = max((int)(__float_as_uint(top) >> 23) - 126, -100);
-          if (need > e + 6) e = need;
           in.ks[lt] = ks * (a.scale * kLog2e);
-          in.vs[lt] = vs * exp2_approx((float)-e);
+          in.vs[lt] = vs;
         }
         if (lane == 0) {
           in.here[lwarp] = word;
-          if (lwarp == 0) { in.all = sound ? 1 : 0; in.e = e; }
+          if (lwarp == 0) in.all = sound ? 1 : 0;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.info_full[inf.s]);

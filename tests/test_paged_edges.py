@@ -55,3 +55,66 @@ def test_heads_of_the_value_cache_must_be_contiguous(op, which, int8):
                 op.paged_attention_decode(x.clone(), x, *pair, table, lengths([1, 1, 1]), 0.1, *scales)
             else:
                 op.paged_attention_chunk(x.clone(), x, *pair, table, lengths([1, 1, 1]), bounds([1, 1, 1]), 0.1, *scales)
+
+
+@pytest.mark.parametrize("size", [2.0 ** 30, 2.0 ** 100, 2.0 ** -60, 0.0])
+@pytest.mark.parametrize("window", [0, 40])
+@pytest.mark.parametrize("hq,hkv,D,dtype", [(4, 2, 128, torch.bfloat16), (3, 1, 64, torch.float16), (16, 1, 96, torch.bfloat16)])
+def test_a_hidden_scale_changes_no_row(op, hq, hkv, D, dtype, window, size):
+    """One K and V scale per token, finite and far from the others: rows that do not see the token keep every bit."""
+    new, total = [230, 3], [700, 80]
+    c = make_cache(total, hkv, D, 16, "token", dtype)
+    q = torch.randn(sum(new), hq, D, device=DEV).to(dtype)
+    out, lse = _attend(op, q, c, total, new, window)
+    group = hq // hkv
+    for pos in (300, 480, 512, 600, 699):                     # in front of every window, in the middle, at a tile's first token, the last
+        w = dict(c, ks=c["ks"].clone(), vs=c["vs"].clone())
+        page, off = _place(c, 0, pos)
+        w["vs"][page, off, 0] = size
+        w["ks"][page, off, 0] = min(size, 2.0 ** 30)
+        out1, lse1 = _attend(op, q, w, total, new, window)
+        for i in range(new[0]):
+            mine = 470 + i
+            if pos > mine or (window and pos <= mine - window):
+                assert torch.equal(out1[i, :group], out[i, :group]) and torch.equal(lse1[i, :group], lse[i, :group]), (pos, i)
+        assert torch.equal(out1[:, group:], out[:, group:]) and torch.equal(out1[new[0]:], out[new[0]:])
+
+
+def _pages(c, n):
+    at = torch.arange(n, device=DEV)
+    return c["tables"][0].long()[at // c["k"].shape[1]], at % c["k"].shape[1]
+
+
+@pytest.mark.parametrize("decode", [True, False])
+@pytest.mark.parametrize("rising", [True, False])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,span", [(700, 13.0), (700, 24.0), (2000, 30.0)])
+def test_scales_over_a_wide_range_by_what_each_row_sees(op, decode, rising, dtype, n, span):
+    """V scales over 2^13 to 2^30 along the positions, the tolerance of each row from the tokens that it sees."""
+    D, hq, hkv = 128, 8, 2
+    new = None if decode else [200]
+    c = make_cache([n], hkv, D, 16, "token", dtype, poison=False)
+    page, off = _pages(c, n)
+    power = torch.linspace(-span / 2, span / 2, n, device=DEV) * (1 if rising else -1)
+    c["vs"][page, off] = (2.0 ** power)[:, None] * 2.0 ** -5
+    q = (torch.randn(1 if decode else 200, hq, D, device=DEV) * 0.3).to(dtype)
+    out, lse = _attend(op, q, c, [n], new)
+    t = q.shape[0]
+    ref, rlse, spread, mass, reach = P.attention(q, c["k"], c["v"], c["tables"], torch.tensor([n]), [0, t], 0.1, c["ks"], c["vs"])
+    # without the part for small weights: that one stands below, from the row's own tokens
+    tol, ltol = attention_tolerance(ref, rlse, spread, torch.zeros_like(mass), reach, D, "token", dtype)
+    K = P.rows_of(c["k"], c["ks"], c["tables"][0], n)
+    code = c["v"][page, off].double().abs()
+    vs = c["vs"][page, off].double()
+    seen = torch.arange(n, device=DEV)[None, :] <= torch.arange(n - t, n, device=DEV)[:, None]
+    for h in range(hq):
+        g = h // (hq // hkv)
+        x = torch.where(seen, 0.1 * (q[:, h].double() @ K[:, g].T), -math.inf)
+        p = torch.softmax(x, -1)
+        # f16 holds the products of weight and scale; below 2^-14 of what they are held relative to, the rounding is absolute, 2^-25.
+        # Decode: relative to at most the row's largest product, which is 1 or more as it is formed.  Chunk: to at
+        # most the largest weight times a power of two that is at most twice the largest scale that the row sees.
+        unit = (p * vs[:, g]).amax(-1) if decode else 2 * torch.where(seen, vs[:, g], 0.0).amax(-1) * p.amax(-1)
+        tol[:, h] += 2.0 ** -25 * unit[:, None] * (seen.double() @ code[:, g])
+    compare(out, ref, tol, "out")
+    compare(lse, rlse, ltol, "lse")
