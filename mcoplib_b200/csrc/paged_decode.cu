@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<T, MODE, DP, NT>::CTAS) decode_k
   const uint32_t block16 = (uint32_t)(a.c.block_stride * C::ELEM / 16), page16 = (uint32_t)(a.c.page_stride * C::ELEM / 16),
                  head16 = (uint32_t)(a.c.head_stride * C::ELEM / 16);
   // Where a lane's pieces of a V row begin.  With FULL these are constants; otherwise pieces behind a row's end read its last
-  // one again (K likewise): the query is zero there, and those rows of O are never written.
+  // one again: those rows of O are never written.  (K is filled up with zeros there: an infinity times the query's zero would be NaN.)
   auto v_piece = [&](int c) { return FULL ? 8 * C::VPIECE * c + C::VPIECE * g : min(8 * C::VPIECE * c + C::VPIECE * g, row_bytes - C::VPIECE); };
 
   // Page and offset of token `lane` of the step at `in`, fetched a step before the copies need them.
@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<T, MODE, DP, NT>::CTAS) decode_k
       const int tok = i * (512 / C::RB > 0 ? 512 / C::RB : 1) + lane / C::ROW16, piece = lane % C::ROW16;
       const char* p = kbase + (uint64_t)__shfl_sync(0xffffffffu, row, tok) * 16;
       cp_async16(dst + tok * C::RB + 16 * (piece ^ (C::RB >= 128 ? (tok & 1) * 4 : 0)), p + (FULL ? 16 * piece : min(16 * piece, row_bytes - 16)),
-                 decltype(all)::value || (ok >> tok & 1));
+                 (decltype(all)::value || (ok >> tok & 1)) && (FULL || 16 * piece < row_bytes));
     }
   };
   auto copy_v = [&](auto all, uint32_t dst, uint32_t row, uint32_t ok) {

@@ -118,3 +118,39 @@ def test_scales_over_a_wide_range_by_what_each_row_sees(op, decode, rising, dtyp
         tol[:, h] += 2.0 ** -25 * unit[:, None] * (seen.double() @ code[:, g])
     compare(out, ref, tol, "out")
     compare(lse, rlse, ltol, "lse")
+
+
+@pytest.mark.parametrize("decode", [True, False])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [16, 48, 64, 80, 96, 128, 144, 256])
+def test_an_infinity_in_k_that_makes_a_logit_minus_infinity(op, D, dtype, decode):
+    """Such a token has weight 0 whatever the head size is padded to; one that a row does not see has no effect at all."""
+    total, hq, hkv = [300, 50], 4, 2
+    new = None if decode else [40, 5]
+    c = make_cache(total, hkv, D, 16, "float", dtype)
+    q = torch.randn(2 if decode else 45, hq, D, device=DEV).to(dtype)
+    q[..., 0] = q[..., 0].abs() + 0.5
+    q[..., -1] = -q[..., -1].abs() - 0.5
+    _, _, _, _, reach = P.attention(q, c["k"], c["v"], c["tables"], torch.tensor(total), bounds(new or [1, 1]).tolist(), 0.1)
+    for pos, d, value in ((7, 0, -math.inf), (100, D - 1, math.inf), (250, D - 1, math.inf)):
+        page, off = _place(c, 0, pos)
+        c["k"][page, off, 0, d] = value
+    out, lse = _attend(op, q, c, total, new)
+    ref, rlse, spread, mass, _ = P.attention(q, c["k"], c["v"], c["tables"], torch.tensor(total), bounds(new or [1, 1]).tolist(), 0.1)
+    tol, ltol = attention_tolerance(ref, rlse, spread, mass, reach, D, "float", dtype)  # (the reach of the finite logits)
+    assert bool(ref.isfinite().all())
+    compare(out, ref, tol, "out")
+    compare(lse, rlse, ltol, "lse")
+
+
+@pytest.mark.parametrize("D", [64, 80, 128, 192])
+def test_decode_takes_no_part_of_hidden_nan_and_infinity(op, D):
+    total, window = [300], 60
+    c = make_cache(total, 2, D, 16, "float", torch.bfloat16)
+    q = torch.randn(1, 8, D, device=DEV).bfloat16()
+    want = _attend(op, q, c, total, window=window)
+    for pos, name, value in ((0, "v", math.nan), (200, "k", math.inf), (239, "v", -math.inf), (238, "k", math.nan)):
+        page, off = _place(c, 0, pos)
+        c[name][page, off, :, D - 3] = value
+    got = _attend(op, q, c, total, window=window)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
