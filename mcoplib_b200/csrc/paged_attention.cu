@@ -101,8 +101,11 @@ int check_args(const char* what, const AttnArgs& a, int64_t tokens, int dtype) {
   MCOP_REQUIRE(a.q_heads > 0 && a.q_heads % a.c.kv_heads == 0, MCOP_ERR_ARGUMENT, "%s: q_heads must be a multiple of kv_heads", what);
   MCOP_REQUIRE(aligned16(a.q) && aligned16(a.out) && a.q_token % 8 == 0 && a.q_head % 8 == 0 && a.o_token % 8 == 0 && a.o_head % 8 == 0,
                MCOP_ERR_ARGUMENT, "%s: query and output rows must be 16-byte aligned", what);
-  MCOP_REQUIRE(a.c.max_blocks >= 0 && a.c.table_stride >= 0 && (int64_t)a.c.max_blocks * a.c.block_size <= INT32_MAX,
-               MCOP_ERR_ARGUMENT, "%s: block table too wide", what);
+  // positions and (token, query head) rows are ints, also rounded up to a tile of up to 256
+  constexpr int64_t kMost = INT32_MAX - 255;
+  MCOP_REQUIRE(a.c.max_blocks >= 0 && a.c.table_stride >= 0 && (int64_t)a.c.max_blocks * a.c.block_size <= kMost, MCOP_ERR_ARGUMENT,
+               "%s: block table too wide", what);
+  MCOP_REQUIRE(tokens * a.q_heads <= kMost, MCOP_ERR_UNSUPPORTED, "%s: more than 2^31 - 256 query rows", what);
   // rows are addressed in units of 16 bytes with 32 bits
   const double span = (double)a.c.num_blocks * a.c.block_stride + (double)a.c.block_size * a.c.page_stride + (double)a.c.kv_heads * a.c.head_stride;
   MCOP_REQUIRE(a.c.block_stride >= 0 && a.c.page_stride >= 0 && a.c.head_stride >= 0 && span * (a.scale_mode ? 1 : 2) < 0x1p36, MCOP_ERR_UNSUPPORTED,
@@ -114,7 +117,6 @@ int check_args(const char* what, const AttnArgs& a, int64_t tokens, int dtype) {
 
 int launch_rows(const char* what, const AttnArgs& a, int dtype, cudaStream_t st) {
   const int64_t ctas = ((int64_t)a.tokens * a.q_heads + 3) / 4;
-  MCOP_REQUIRE(ctas <= INT32_MAX, MCOP_ERR_UNSUPPORTED, "%s: too many tokens", what);
   auto go = [&](auto kernel) {
     launch_pdl(kernel, dim3((unsigned)ctas), dim3(128), 0, st, a);
     return check_launch(what);

@@ -1084,8 +1084,7 @@ int launch_chunk(const AttnArgs& a, int dtype, void* ws, size_t ws_bytes, cudaSt
   MCOP_REQUIRE(ws && aligned16(ws) && ws_bytes >= chunk_workspace(a.tokens, a.batch, a.q_heads, a.c.kv_heads, a.head_size), MCOP_ERR_WORKSPACE,
                "%s: workspace missing, misaligned or too small", what);
   const double span = (double)a.tokens * a.q_token + (double)a.q_heads * a.q_head;
-  MCOP_REQUIRE((int64_t)a.tokens * a.q_heads <= INT32_MAX && a.q_token >= 0 && a.q_head >= 0 && span < 0x1p34, MCOP_ERR_UNSUPPORTED,
-               "%s: more than 2^31 query rows, or a query that spans more than 2^34 elements", what);
+  MCOP_REQUIRE(a.q_token >= 0 && a.q_head >= 0 && span < 0x1p34, MCOP_ERR_UNSUPPORTED, "%s: a query that spans more than 2^34 elements", what);
   return dtype == MCOP_BF16 ? launch_type<__nv_bfloat16>(a, ws, st) : launch_type<__half>(a, ws, st);
 }
 
