@@ -255,7 +255,9 @@ int mcop_reshape_and_cache_dynamic_i8(const void* key, const void* value, int64_
 /* Read a batch of sequences back out of the cache.  No counterpart in the reference.
  * key_out, value_out [tokens, kv_heads, head_size] contiguous: row cu_seq_lens[b] + p = position p of sequence b, times its
  * scale, rounded once to dtype (bf16, f16; f32 with an int8 cache; dtype is the cache's own type with scale_mode 0).
- * cu_seq_lens int32 [batch + 1].  Rows before cu_seq_lens[0], behind cu_seq_lens[batch] and of bad pages keep what they held. */
+ * cu_seq_lens int32 [batch + 1].  Rows before cu_seq_lens[0], behind cu_seq_lens[batch], of bad pages and of
+ * sequences that leave the buffer keep what they held; where bounds descend (MCOP_DEVERR_SEQUENCE), a row that several sequences
+ * claim gets the row of one of them. */
 int mcop_gather_and_dequant_cache(void* key_out, void* value_out, const void* key_cache, const void* value_cache,
                                   int64_t block_stride, int64_t page_stride, int64_t head_stride, const float* k_scale,
                                   const float* v_scale, int scale_mode, const int32_t* block_tables, int64_t table_stride,

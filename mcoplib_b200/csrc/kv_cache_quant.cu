@@ -110,22 +110,25 @@ __global__ void __launch_bounds__(256) kv_quant_store_kernel(const T* __restrict
 // The sequence is found by a 32-way search (one ballot per level: a batch of up to 31 needs one load), then the warp walks
 // the token's kv_heads * head_size elements of K and V, 16 per lane.
 // Rows behind cu[batch] are left as they were; a row whose page is not in the table or not in the cache likewise, and
-// it is reported.
+// it is reported.  So are the rows of a sequence that leaves the buffer.  One CTA behind the others looks all bounds over and reports
+// those that descend or leave the buffer (a sequence without rows leads no warp to its bounds).
 // ---------------------------------------------------------------------------------------------
 template <typename T, bool I8>
 __global__ void __launch_bounds__(256) kv_gather_kernel(T* __restrict__ key_out, T* __restrict__ value_out, PagedCache c, int scale_mode,
                                                         const int32_t* __restrict__ cu, int batch, int64_t tokens, int head_size, int* err) {
   pdl_launch_dependents();
   pdl_wait();
+  if (blockIdx.x == gridDim.x - 1) {
+    for (int b = threadIdx.x; b < batch; b += 256)
+      if (cu[b] < 0 || cu[b + 1] < cu[b] || cu[b + 1] > tokens) report(err, MCOP_DEVERR_SEQUENCE);
+    return;
+  }
   const int lane = threadIdx.x & 31;
   const int64_t t = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (t >= tokens || t < cu[0] || t >= cu[batch]) return;
-  const int b = find_sequence(cu, batch, t);
+  const int b = find_sequence(cu, batch, t);  // cu[b] <= t < cu[b + 1], whatever the others are
   const int64_t pos = t - cu[b];
-  if (pos < 0) {  // the bounds are not ascending
-    if (lane == 0) report(err, MCOP_DEVERR_SEQUENCE);
-    return;
-  }
+  if (pos > t || cu[b + 1] > tokens) return;  // the sequence leaves the buffer
   const int64_t page = pos / c.block_size;
   const int64_t block = page < c.max_blocks ? c.tables[b * c.table_stride + page] : -1;
   if (block < 0 || block >= c.num_blocks) {
@@ -257,7 +260,7 @@ extern "C" int mcop_gather_and_dequant_cache(void* key_out, void* value_out, con
   MCOP_REQUIRE(aligned16(key_out) && aligned16(value_out), MCOP_ERR_ARGUMENT, "%s: outputs must be 16-byte aligned", what);
   MCOP_REQUIRE(max_blocks >= 0 && table_stride >= 0 && block_stride >= 0 && page_stride >= 0 && head_stride >= 0, MCOP_ERR_ARGUMENT,
                "%s: bad stride", what);
-  const int64_t ctas = (tokens + 7) / 8;
+  const int64_t ctas = (tokens + 7) / 8 + 1;
   MCOP_REQUIRE(ctas <= INT32_MAX, MCOP_ERR_UNSUPPORTED, "%s: too many tokens", what);
   PagedCache c{key_cache, value_cache, k_scale, v_scale, block_stride, page_stride, head_stride, block_tables, table_stride, max_blocks,
                block_size, num_blocks, kv_heads};

@@ -154,3 +154,35 @@ def test_decode_takes_no_part_of_hidden_nan_and_infinity(op, D):
         c[name][page, off, :, D - 3] = value
     got = _attend(op, q, c, total, window=window)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("kind", ["float", "token"])
+@pytest.mark.parametrize("cu,kept", [
+    ([0, 30, 20, 40], [(40, 50)]),              # descends: sequence 1 has no rows, 0 and 2 overlap
+    ([-4, 10, 20, 30], [(0, 10), (30, 50)]),    # begins in front of the buffer: sequence 0 is left out
+    ([0, 10, 20, 60], [(20, 50)]),              # ends behind it: sequence 2 is left out
+    ([0, 10, 60, 70], [(10, 50)]),
+])
+def test_read_back_leaves_out_and_reports_sequences_outside_the_buffer(op, kind, cu, kept):
+    c = make_cache([64, 64, 64], 2, 64, 16, kind, torch.bfloat16, poison=False)
+    out = [torch.full((50, 2, 64), 7.0, device=DEV).bfloat16() for _ in range(2)]
+    op.gather_and_dequant_cache(*out, c["k"], c["v"], c["tables"], torch.tensor(cu, dtype=torch.int32, device=DEV), c["ks"], c["vs"])
+    assert cabi.load().mcop_device_error() == cabi.DEVERR_SEQUENCE
+    untouched = torch.zeros(50, dtype=torch.bool, device=DEV)
+    for a, b in kept:
+        untouched[a:b] = True
+    for o, cache, scale in zip(out, (c["k"], c["v"]), (c["ks"], c["vs"])):
+        assert bool((o[untouched] == 7).all())
+        rows = [P.rows_of(cache, scale, c["tables"][b], 64).float().bfloat16() for b in range(3)]
+        for t in torch.nonzero(~untouched).flatten().tolist():
+            mine = [rows[b][t - cu[b]] for b in range(3) if 0 <= cu[b] <= t < cu[b + 1] <= 50]
+            assert any(torch.equal(o[t], r) for r in mine), t
+
+
+def test_read_back_reports_bad_bounds_that_no_row_meets(op):
+    c = make_cache([5] * 700, 1, 32, 16, "float", torch.bfloat16, poison=False)
+    cu = bounds([0] * 650 + [5] * 50)
+    cu[300] = -1                                              # an empty sequence in front of the buffer, one that descends
+    out = [torch.empty(250, 1, 32, device=DEV).bfloat16() for _ in range(2)]
+    op.gather_and_dequant_cache(*out, c["k"], c["v"], c["tables"], cu)
+    assert cabi.load().mcop_device_error() == cabi.DEVERR_SEQUENCE
