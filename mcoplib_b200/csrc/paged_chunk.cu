@@ -402,12 +402,6 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
         const Info& in = info[inf.s];
         if (!(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&bars.info_full[inf.s], inf.phase, a.err, kWaitSoftmax, kSpin)))) break;
         inf.advance(C::NI);
-        const int base = (pt.first + k) * kTile;
-        const bool masked = __any_sync(0xffffffffu, base < lo || base + kTile > hi) || !in.all;
-        auto seen_of = [&](int i) {  // columns [lo - base, hi - base) of [32 i, 32 i + 32) that are there
-          const int f = min(32, max(0, lo - base - 32 * i)), e = min(32, max(0, hi - base - 32 * i));
-          return (uint32_t)((1ull << e) - 1) & ~(uint32_t)((1ull << f) - 1) & in.here[i];
-        };
         if (!(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&bars.s_full[group], s_phase, a.err, kWaitSoftmax, kSpin)))) break;
         s_phase ^= 1;
         tc_fence_after();
@@ -421,6 +415,12 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
 #pragma unroll
           for (int i = 0; i < 128; ++i) s[i] = -s[i];
         }
+        const int base = (pt.first + k) * kTile;
+        const bool masked = __any_sync(0xffffffffu, base < lo || base + kTile > hi) || !in.all;
+        auto seen_of = [&](int i) {  // columns [lo - base, hi - base) of [32 i, 32 i + 32) that are there
+          const int f = min(32, max(0, lo - base - 32 * i)), e = min(32, max(0, hi - base - 32 * i));
+          return (uint32_t)((1ull << e) - 1) & ~(uint32_t)((1ull << f) - 1) & in.here[i];
+        };
         // factors of the columns; where columns are hidden, the products with them are formed here
         uint32_t factor = 0, vfactor = 0;
         bool wild = false;
