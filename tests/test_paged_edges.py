@@ -186,3 +186,20 @@ def test_read_back_reports_bad_bounds_that_no_row_meets(op):
     out = [torch.empty(250, 1, 32, device=DEV).bfloat16() for _ in range(2)]
     op.gather_and_dequant_cache(*out, c["k"], c["v"], c["tables"], cu)
     assert cabi.load().mcop_device_error() == cabi.DEVERR_SEQUENCE
+
+
+def test_store_of_fp32_rows_from_the_smallest_to_infinity(op):
+    """Subnormal scales, rows near the largest float, and rows that hold infinities or NaN: scale NaN, codes 0, which equal only themselves."""
+    g = torch.Generator(device=DEV).manual_seed(3)
+    size = torch.tensor([0.0, 1e-44, 1e-42, 1e-38, 1e-36, 1.0, 1e30, 1e38, 1e38, 3e38], device=DEV)
+    key, value = (torch.randn(10, 3, 48, generator=g, device=DEV).clamp(-1, 1) * size[:, None, None] for _ in range(2))
+    value[8, 0, 5], value[8, 2, 47], key[9, 1, 0] = math.inf, -math.inf, math.nan
+    kc, vc = (torch.full((2, 5, 3, 48), 9, dtype=torch.int8, device=DEV) for _ in range(2))
+    ks, vs = (torch.full((2, 5, 3), 9.0, device=DEV) for _ in range(2))
+    ref = [x.clone() for x in (kc, vc, ks, vs)]
+    slots = torch.randperm(10, generator=g, device=DEV)
+    P.store(key, value, *ref, slots)
+    op.reshape_and_cache_dynamic_int8(key, value, kc, vc, ks, vs, slots)
+    for got, want in zip((kc, vc, ks, vs), ref):
+        assert bool(((got == want) | (got.isnan() & want.isnan())).all())
+    assert int(ref[2].isnan().sum()) == 1 and int(ref[3].isnan().sum()) == 2
