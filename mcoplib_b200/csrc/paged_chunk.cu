@@ -88,6 +88,20 @@ __device__ __forceinline__ Reach reach(const AttnArgs& a, const Seq& s, int t, i
   return r;
 }
 
+// Tokens [lo, hi) that all rows of a query tile see: 128 tokens inside need no care for what a row must not see.
+struct Common {
+  int lo, hi;
+  __device__ __forceinline__ bool whole(int base) const { return base >= lo && base + kTile <= hi; }
+};
+__device__ __forceinline__ Common seen_by_all(const AttnArgs& a, const PlanTile& pt, int group) {
+  const Seq s{pt.q0, pt.qn, pt.len};
+  Common c;
+  int other;
+  span(a, s, (pt.t * kRows + pt.rows - 1) / group, c.lo, other);
+  span(a, s, pt.t * kRows / group, other, c.hi);
+  return c;
+}
+
 __global__ void __launch_bounds__(1024) chunk_plan_kernel(AttnArgs a, Layout w, int64_t limit, int ctas) {
   pdl_launch_dependents();
   pdl_wait();
@@ -589,19 +603,26 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
             if (lane == 0) mbar_arrive(&bars.o_empty[group]);
           }
           if constexpr (!C::I8) {
-            if (sick && mine) {  // the masked tiles were added up without their NaNs and infinities: add those that this row sees
+            if (sick && mine) {  // the tiles that some rows see in part were added up without their NaNs and infinities: add those that this row sees
+              const Common common = seen_by_all(a, pt, G);
               for (int k = x.k0; k < x.k1; ++k) {
                 const int base = (pt.first + k) * kTile;
+                if (common.whole(base)) continue;
                 for (int j = max(lo, base); j < min(hi, base + kTile); ++j) {
                   const int slot = slot_of(a, pt.b, j);
                   if (slot < 0) continue;
                   const T* v = static_cast<const T*>(a.c.v) + row_of(a.c, slot, x.head) + 32 * i;
-                  for (int d = 0; d < 32 && 32 * i + d < a.head_size; ++d) {
-                    const float y = ElemTraits<T>::to_float(v[d]);
-                    if (!(fabsf(y) <= FLT_MAX)) {
 #pragma unroll
-                      for (int z = 0; z < 32; ++z)
-                        if (z == d) o[z] += y;
+                  for (int d = 0; d < 32; d += 8) {
+                    if (32 * i + d >= a.head_size) break;
+                    const uint4 u = *reinterpret_cast<const uint4*>(v + d);
+                    uint4 clean = u;
+                    if (!not_finite<T>(clean)) continue;
+                    const T* y = reinterpret_cast<const T*>(&u);
+#pragma unroll
+                    for (int z = 0; z < 8; ++z) {
+                      const float x = ElemTraits<T>::to_float(y[z]);
+                      if (!(fabsf(x) <= FLT_MAX)) o[d + z] += x;
                     }
                   }
                 }
@@ -722,11 +743,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
     while (x.next(w, a.c.kv_heads, pt)) {
       if (lt == 0) *(volatile int*)&poison[item & 7] = 0;
       // rows of Q
-      const Seq seq{pt.q0, pt.qn, pt.len};
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int row = lt + 128 * i, flat = pt.t * kRows + row, token = flat / G;
-        q_at[row] = row < pt.rows ? (uint32_t)(((int64_t)(seq.q0 + token) * a.q_token + (int64_t)(x.head * G + flat - token * G) * a.q_head) / 8) : 0xffffffffu;
+        q_at[row] = row < pt.rows ? (uint32_t)(((int64_t)(pt.q0 + token) * a.q_token + (int64_t)(x.head * G + flat - token * G) * a.q_head) / 8) : 0xffffffffu;
       }
       if (item > 0) {
         ok = ok && acquire(&bars.q_empty, q_phase);
@@ -742,10 +762,6 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
                      live ? static_cast<const T*>(a.q) + (int64_t)at * 8 + c * 8 : static_cast<const T*>(a.q), live);
         }
       }
-      // tokens that all rows of the item see: tiles inside need no care for what a row must not see
-      int all_lo, all_hi, other;
-      span(a, seq, (pt.t * kRows + pt.rows - 1) / G, all_lo, other);
-      span(a, seq, pt.t * kRows / G, other, all_hi);
       // page of token `lt` of a tile, fetched a tile ahead
       int block = -1, off = -1;
       auto look_up = [&](int k) {
@@ -815,10 +831,11 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
         look_up(k + 1);
       };
       if constexpr (!C::I8) {
+        const Common common = seen_by_all(a, pt, G);
         for (int k = x.k0; k < x.k1; ++k) {
           prepare(k);
           const int base = (pt.first + k) * kTile;
-          const bool scan = base < all_lo || base + kTile > all_hi;
+          const bool scan = !common.whole(base);
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
             const char* src = kv ? vbase : kbase;

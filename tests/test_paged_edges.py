@@ -203,3 +203,29 @@ def test_store_of_fp32_rows_from_the_smallest_to_infinity(op):
     for got, want in zip((kc, vc, ks, vs), ref):
         assert bool(((got == want) | (got.isnan() & want.isnan())).all())
     assert int(ref[2].isnan().sum()) == 1 and int(ref[3].isnan().sum()) == 2
+
+
+@pytest.mark.parametrize("window", [0, 500])
+def test_nan_and_infinity_in_a_long_context(op, window):
+    """Non-finite elements of V in tiles that all rows of an item see, and in those that some see, thousands of tokens in."""
+    new, total, hq, hkv, D = [300], [6000], 4, 2, 128
+    c = make_cache(total, hkv, D, 16, "float", torch.bfloat16)
+    q = torch.randn(300, hq, D, device=DEV).bfloat16()
+    good, lse0 = _attend(op, q, c, total, new, window)
+    special = [(64, 9, math.inf), (5400, 9, -math.inf), (5820, 40, math.inf), (5990, 77, math.nan), (5999, 127, -math.inf)]
+    for pos, d, value in special:
+        page, off = _place(c, 0, pos)
+        c["v"][page, off, 0, d] = value
+    out, lse = _attend(op, q, c, total, new, window)
+    assert torch.equal(lse, lse0) and torch.equal(out[:, 2:], good[:, 2:])
+    for i in range(300):
+        mine = 5700 + i
+        hit = {}
+        for pos, d, value in special:
+            if pos <= mine and (not window or pos > mine - window):
+                hit[d] = hit.get(d, 0.0) + value              # inf - inf is NaN, as in the sum itself
+        want = good[i, :2].float()
+        for d, value in hit.items():
+            want[:, d] = value
+        assert torch.equal(torch.nan_to_num(out[i, :2].float(), nan=-5.0, posinf=1e30, neginf=-1e30),
+                           torch.nan_to_num(want, nan=-5.0, posinf=1e30, neginf=-1e30)), i
