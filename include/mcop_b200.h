@@ -269,6 +269,8 @@ int mcop_gather_and_dequant_cache(void* key_out, void* value_out, const void* ke
  * query head h reads KV head h / (q_heads / kv_heads).  The token of sequence b is its last cached one: it sees the last
  * `window` positions (0: all) of [0, seq_lens[b]).  out = softmax(scale * q . k) v; lse (fp32 [batch, q_heads], may be NULL)
  * = ln sum exp(scale * q . k).  A sequence of length 0 gets out = 0 and lse = -inf.  scale must be positive.
+ * V scales per token are meant to lie within 2^-90 and 2^100 in size, or be 0: smaller ones lose bits of out, above 2^100 the
+ * products of weight and scale overflow.
  * The lengths stay on the device, so one captured graph serves any lengths.  workspace: 16-byte aligned, at least
  * mcop_paged_attention_decode_workspace_bytes(); needs no initialisation, must not be shared by calls that overlap. */
 size_t mcop_paged_attention_decode_workspace_bytes(int batch, int q_heads, int kv_heads, int head_size);

@@ -406,8 +406,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<T, MODE, DP, NT>::CTAS) decode_k
           if constexpr (MODE == kScaleToken) {
             ks = scales[tok];
             vs[hf][r] = scales[C::TOK + tok];
-            // what a token's scale adds to its logit where the maximum is concerned (bounded, so that fp32 holds the weights' sum)
-            ref[hf][r] = __log2f(fminf(fmaxf(fabsf(vs[hf][r]), 0x1p-60f), 0x1p60f));
+            // what a token's scale adds to its logit where the maximum is concerned (bounded, so that fp32 holds the weights and their
+            // sum: 2^29 weights of 2^(90 + 8), and weights down to 2^-26 of the largest beside a scale of 2^100)
+            ref[hf][r] = __log2f(fminf(fmaxf(fabsf(vs[hf][r]), 0x1p-90f), 0x1p100f));
           }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {

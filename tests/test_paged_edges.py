@@ -229,3 +229,22 @@ def test_nan_and_infinity_in_a_long_context(op, window):
             want[:, d] = value
         assert torch.equal(torch.nan_to_num(out[i, :2].float(), nan=-5.0, posinf=1e30, neginf=-1e30),
                            torch.nan_to_num(want, nan=-5.0, posinf=1e30, neginf=-1e30)), i
+
+
+@pytest.mark.parametrize("decode", [True, False])
+@pytest.mark.parametrize("power", [-85, -62, 40, 62, 90])
+def test_v_scales_of_any_size(op, decode, power):
+    """All V scales times a power of two: the output takes it over, the log-sum-exp knows nothing of it."""
+    total, D = [900, 33], 128
+    new = None if decode else [70, 33]
+    c = make_cache(total, 2, D, 16, "token", torch.bfloat16, poison=False)
+    q = (torch.randn(2 if decode else 103, 8, D, device=DEV) * 0.3).bfloat16()
+    c["vs"] *= 2.0 ** power
+    out, lse = _attend(op, q, c, total, new)
+    cu = bounds(new or [1, 1]).tolist()
+    ref, rlse, spread, mass, reach = P.attention(q, c["k"], c["v"], c["tables"], torch.tensor(total), cu, 0.1, c["ks"], c["vs"])
+    tol, ltol = attention_tolerance(ref, rlse, spread, mass, reach, D, "token", torch.bfloat16)
+    # Weights are formed as 2^(x - r) with |r| <= 128: rounding the exponent moves them by at most 2^-18 * ln 2, half a step of a number
+    # below 128, and log2 of their sum, below 128 in size, is off by two such steps
+    compare(out, ref, tol + 2.0 ** -18 * spread, "out")
+    compare(lse, rlse, ltol + 2.0 ** -16, "lse")
