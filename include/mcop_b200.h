@@ -54,7 +54,8 @@ enum {
   MCOP_DEVERR_WAIT_LAST = 15,
   MCOP_DEVERR_POSITION = 16, /* RoPE position outside [0, max_position) */
   MCOP_DEVERR_SLOT = 17,     /* paged-cache slot >= num_blocks * block_size */
-  MCOP_DEVERR_KV_INDEX = 18, /* store_kv: slot id outside [0, num_slots) or cache position outside [0, max_len) */
+  MCOP_DEVERR_KV_INDEX = 18, /* store_kv: slot id outside [0, num_slots) or cache position outside [0, max_len); paged cache: a
+                                sequence longer than its row of the block table, or of negative length */
   MCOP_DEVERR_SEQUENCE = 19, /* sequence bounds that descend or leave the buffer */
   MCOP_DEVERR_SELFTEST = 99  /* recorded by mcop_selftest_wait_timeout */
 };
@@ -254,7 +255,8 @@ int mcop_reshape_and_cache_dynamic_i8(const void* key, const void* value, int64_
 
 /* Read a batch of sequences back out of the cache.  No counterpart in the reference.
  * key_out, value_out [tokens, kv_heads, head_size] contiguous: row cu_seq_lens[b] + p = position p of sequence b, times its
- * scale, rounded once to dtype (bf16, f16; f32 with an int8 cache; dtype is the cache's own type with scale_mode 0).
+ * scale, the product rounded to fp32 and then to dtype (bf16, f16; f32 with an int8 cache; dtype is the cache's own type with
+ * scale_mode 0: a copy).
  * cu_seq_lens int32 [batch + 1].  Rows before cu_seq_lens[0], behind cu_seq_lens[batch], of bad pages and of
  * sequences that leave the buffer keep what they held; where bounds descend (MCOP_DEVERR_SEQUENCE), a row that several sequences
  * claim gets the row of one of them. */

@@ -106,7 +106,8 @@ __global__ void __launch_bounds__(256) kv_quant_store_kernel(const T* __restrict
 }
 
 // ---------------------------------------------------------------------------------------------
-// Read-back: row t of sequence b (cu[b] <= t < cu[b + 1]) = T(cached row * scale), one rounding.  One warp per token.
+// Read-back: row t of sequence b (cu[b] <= t < cu[b + 1]) = T(fp32(cached row * scale)): the product has up to 31 bits, is rounded to fp32
+// and then to T, as the same expression on fp32 tensors is.  One warp per token.
 // The sequence is found by a 32-way search (one ballot per level: a batch of up to 31 needs one load), then the warp walks
 // the token's kv_heads * head_size elements of K and V, 16 per lane.
 // Rows behind cu[batch] are left as they were; a row whose page is not in the table or not in the cache likewise, and

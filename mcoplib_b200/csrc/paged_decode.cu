@@ -3,7 +3,8 @@
 // Bound: HBM bytes of the cached rows (all query heads of a KV head share its rows).  16 * head_size flops per row byte
 // (int8, 8 query heads per KV head) is more than the fp32 pipes give at the memory's rate, so both products run on the
 // tensor cores with TOKENS as the M dimension: m16n8k16 takes 16 cached tokens against 8 query heads, which wastes nothing at
-// 8 heads per KV head (a 128-row tcgen05 tile would be 1/16 full, and its M is the query side).
+// 8 heads per KV head.  (tcgen05.mma could take 128 tokens against 8 heads as well; it would want K and V, converted, in swizzled
+// shared memory, where mma.sync takes them from registers as they arrive.  Not built.)
 //   S^T[16 tokens x 8 heads] = K[16 x D] Q^T[D x 8]         O^T[D x 8] += V^T[D x 16] P^T[16 x 8]
 // The order of the contracted index is free as long as both operands agree, and so is the order of O's rows: a lane's
 // fragments are 16-byte pieces of cached rows as they lie, int8 codes become f16 in registers (exactly), and the only
