@@ -85,6 +85,21 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+// 16 bytes to shared memory, or 16 zeros (nothing is read then).
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+// Two floats rounded to T, lo in the low half.
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (ElemTraits<T>::code == MCOP_BF16) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&h);
+  } else {
+    __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&h);
+  }
+}
+
 // Decode (paged_decode.cu): one new token per sequence, head sizes up to 256.
 size_t decode_workspace(int q_heads, int kv_heads, int head_size);
 int launch_decode(const AttnArgs& a, int dtype, void* ws, size_t ws_bytes, cudaStream_t st);

@@ -208,9 +208,6 @@ struct WorkLine {
   }
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
-}
 __device__ __forceinline__ void sts_u4(uint32_t dst, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
@@ -232,15 +229,6 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
   return ok != 0;
 }
 __device__ __forceinline__ void async_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  if constexpr (ElemTraits<T>::code == MCOP_BF16) {
-    __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<uint32_t*>(&h);
-  } else {
-    __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<uint32_t*>(&h);
-  }
-}
 // Two codes (bytes 0 and 2 of x, the others ignored) as a pair of T, exactly: 128 + seven bits minus 128 or 256 in bf16, 1024 +
 // (code + 128) in f16.  The masks stay in registers: as immediates each would cost an instruction of its own.
 struct Codes {
@@ -510,8 +498,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(AttnArgs a, Layout w
           m = to;
           l *= keep;
           if (k > x.k0) {
-            // (S of this tile was issued behind the previous tile's P V: that product is complete)
-// (8 columns at a time: the logits stay in registers meanwhile)
+            // (S of this tile was issued behind the previous tile's P V: that product is complete.  8 columns at a time: the logits
+            // stay in registers meanwhile)
 #pragma unroll 1
             for (int i = 0; i < DP; i += 8) {
               float o[8];
