@@ -235,7 +235,8 @@ int mcop_rope_kv_store_i8_paged(const int64_t* positions, void* query, void* key
  * [kv_heads] (what mcop_rope_kv_store_i8_paged writes); 2: int8 with k_scale, v_scale fp32 [num_blocks, block_size, kv_heads]
  * (what mcop_reshape_and_cache_dynamic_i8 writes).  value = code * scale.
  * block_tables int32 [batch, table_stride], of whose rows the first max_blocks entries count: position p of sequence b is
- * at offset p % block_size of block block_tables[b, p / block_size].  Entries behind a sequence's last page are not read.
+ * at offset p % block_size of block block_tables[b, p / block_size].  Entries behind a sequence's last page are not read (block_tables
+ * may be NULL with max_blocks 0, where nothing is cached).
  * The attention operators take tables of at most 2^31 - 256 positions and at most 2^31 - 256 (token, query head) rows.
  * A page outside [0, num_blocks) hides its tokens (MCOP_DEVERR_SLOT), a length beyond the table is cut (MCOP_DEVERR_KV_INDEX),
  * a sequence whose bounds descend or leave the buffer is skipped (MCOP_DEVERR_SEQUENCE).

@@ -250,7 +250,7 @@ extern "C" int mcop_gather_and_dequant_cache(void* key_out, void* value_out, con
   const char* what = "gather_and_dequant_cache";
   MCOP_REQUIRE(tokens >= 0 && batch >= 0, MCOP_ERR_ARGUMENT, "%s: negative size", what);
   if (tokens == 0 || batch == 0) return MCOP_OK;
-  MCOP_REQUIRE(key_out && value_out && key_cache && value_cache && block_tables && cu_seq_lens, MCOP_ERR_ARGUMENT, "%s: null pointer", what);
+  MCOP_REQUIRE(key_out && value_out && key_cache && value_cache && (block_tables || max_blocks == 0) && cu_seq_lens, MCOP_ERR_ARGUMENT, "%s: null pointer", what);
   MCOP_REQUIRE(scale_mode >= kScaleNone && scale_mode <= kScaleToken && (scale_mode == kScaleNone || (k_scale && v_scale)), MCOP_ERR_ARGUMENT,
                "%s: scales missing", what);
   const bool i8 = scale_mode != kScaleNone;

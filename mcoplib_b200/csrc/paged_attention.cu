@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(128) attention_rows_kernel(AttnArgs a) {
 }
 
 int check_args(const char* what, const AttnArgs& a, int64_t tokens, int dtype) {
-  MCOP_REQUIRE(a.q && a.out && a.c.k && a.c.v && a.c.tables && a.seq_lens, MCOP_ERR_ARGUMENT, "%s: null pointer", what);
+  MCOP_REQUIRE(a.q && a.out && a.c.k && a.c.v && (a.c.tables || a.c.max_blocks == 0) && a.seq_lens, MCOP_ERR_ARGUMENT, "%s: null pointer", what);
   MCOP_REQUIRE(tokens <= INT32_MAX, MCOP_ERR_UNSUPPORTED, "%s: too many tokens", what);
   MCOP_REQUIRE(dtype == MCOP_BF16 || dtype == MCOP_F16, MCOP_ERR_UNSUPPORTED, "%s: query must be bf16 or f16", what);
   MCOP_REQUIRE(a.scale_mode >= kScaleNone && a.scale_mode <= kScaleToken && (a.scale_mode == kScaleNone || (a.c.k_scale && a.c.v_scale)),

@@ -248,3 +248,18 @@ def test_v_scales_of_any_size(op, decode, power):
     # below 128, and log2 of their sum, below 128 in size, is off by two such steps
     compare(out, ref, tol + 2.0 ** -18 * spread, "out")
     compare(lse, rlse, ltol + 2.0 ** -16, "lse")
+
+
+@pytest.mark.parametrize("kind", ["float", "token"])
+@pytest.mark.parametrize("D", [64, 192])
+def test_a_table_without_columns(op, kind, D):
+    """Nothing is cached yet: a table of no pages per sequence is as good as an unused one."""
+    c = make_cache([0, 0, 0], 2, D, 16, kind, torch.bfloat16)
+    c["tables"] = torch.empty(3, 0, dtype=torch.int32, device=DEV)
+    for new in (None, [2, 0, 3]):
+        q = torch.randn(3 if new is None else 5, 4, D, device=DEV).bfloat16()
+        out, lse = _attend(op, q, c, [0, 0, 0], new)
+        assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+    rows = [torch.full((4, 2, D), 7.0, device=DEV).bfloat16() for _ in range(2)]
+    op.gather_and_dequant_cache(*rows, c["k"], c["v"], c["tables"], bounds([0, 0, 0]), c["ks"], c["vs"])
+    assert bool((rows[0] == 7).all()) and bool((rows[1] == 7).all()) and cabi.load().mcop_device_error() == 0
